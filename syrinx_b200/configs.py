@@ -79,6 +79,96 @@ class SxCodecInfo(C.Structure):
     ]
 
 
+class SxPagedCache(C.Structure):
+    """sx_paged_cache of include/syrinx_paged.h."""
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("page_stride", C.c_int64),
+        ("head_stride", C.c_int64),
+        ("token_stride", C.c_int64),
+        ("dtype", C.c_int32),
+        ("n_pages", C.c_int32),
+        ("page_size", C.c_int32),
+        ("n_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class SxPagedPlanArgs(C.Structure):
+    """sx_paged_plan_args of include/syrinx_paged.h."""
+    _fields_ = [
+        ("lens_in", C.c_void_p),
+        ("delta", C.c_void_p),
+        ("n_free_in", C.c_void_p),
+        ("lens_out", C.c_void_p),
+        ("n_free_out", C.c_void_p),
+        ("table", C.c_void_p),
+        ("free_pages", C.c_void_p),
+        ("slots", C.c_void_p),
+        ("tok_seq", C.c_void_p),
+        ("tok_pos", C.c_void_p),
+        ("starts", C.c_void_p),
+        ("status", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("table_width", C.c_int32),
+        ("n_req", C.c_int32),
+        ("n_pages", C.c_int32),
+        ("page_size", C.c_int32),
+        ("max_tokens", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class SxPagedAppendArgs(C.Structure):
+    """sx_paged_append_args of include/syrinx_paged.h."""
+    _fields_ = [
+        ("cache", SxPagedCache),
+        ("x", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("slots", C.c_void_p),
+        ("positions", C.c_void_p),
+        ("cos", C.c_void_p),
+        ("sin", C.c_void_p),
+        ("q_norm", C.c_void_p),
+        ("k_norm", C.c_void_p),
+        ("status", C.c_void_p),
+        ("x_stride", C.c_int64),
+        ("q_stride", C.c_int64),
+        ("eps", C.c_float),
+        ("x_dtype", C.c_int32),
+        ("n_rows", C.c_int32),
+        ("n_heads", C.c_int32),
+        ("n_positions", C.c_int32),
+        ("interleaved", C.c_int32),
+    ]
+
+
+class SxPagedAttentionArgs(C.Structure):
+    """sx_paged_attention_args of include/syrinx_paged.h."""
+    _fields_ = [
+        ("cache", SxPagedCache),
+        ("q", C.c_void_p),
+        ("out", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("table", C.c_void_p),
+        ("lens", C.c_void_p),
+        ("status", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+        ("q_stride", C.c_int64),
+        ("out_stride", C.c_int64),
+        ("table_stride", C.c_int64),
+        ("table_width", C.c_int32),
+        ("n_req", C.c_int32),
+        ("n_heads", C.c_int32),
+        ("q_dtype", C.c_int32),
+        ("max_len", C.c_int32),
+        ("scale", C.c_float),
+    ]
+
+
 @dataclasses.dataclass(frozen=True)
 class Stack:
     dim: int
