@@ -1,12 +1,34 @@
 // paged_attention.cu — attention of one new token per request over its pages
 // (sx_paged_attention).
 //
-// One CTA of 8 warps per (request, kv head). Each warp takes every eighth key: lanes split the
-// head dimension, the scores of the group's query heads are shuffle sums, and a running
-// maximum m, sum l and output o per head fold the keys in one pass:
-//   m' = max(m, s), l' = l 2^(m - m') + 2^(s - m'), o' = o 2^(m - m') + 2^(s - m') v,
-// with s in units of log 2. The warps' (m, l, o) are joined the same way through shared memory.
+// Mathematics. With scores in units of log 2, s_t = scale log2(e) q.k_t, one pass over the keys
+// keeps a running maximum m, sum l and output o per query head:
+//   m' = max(m, s), l' = l 2^(m - m') + 2^(s - m'), o' = o 2^(m - m') + 2^(s - m') v;
+// partial results over disjoint keys join by the same rule. out = o / l, lse = ln 2 (m + log2 l).
+//
+// Bound. Every key and value is read once for its whole group of query heads: 2 len Hkv hd
+// elements per request, a few operations each, so the kernel is bound by HBM when there is
+// enough to read and by latency when there is not.
+//
+// Split. The keys of every (request, kv head) are cut into tiles of 8 KB (16 keys of 128 bf16
+// elements); all tiles of the batch, request by request and head by head, are one line that is
+// cut into even shares, one per CTA (one CTA per SM), and a CTA's share into even runs, one per
+// warp. However uneven the lengths are, every SM reads the same number of bytes. A warp copies
+// its own tiles into a ring of its own (cp.async), so nothing in the main loop waits for
+// another warp, and the ring runs on across the end of one request and the start of the next.
+// A (request, kv head) that lies inside one warp's run is finished by that warp; runs that
+// begin or end inside one leave a partial (m, l, o), joined in shared memory at the end of the
+// CTA, and, where a share begins or ends inside one, through the workspace by a second kernel.
+// Every partial is joined in key order, so results repeat bit for bit.
+//
+// Products. 16-bit pages: mma.sync.m16n8k16 with the keys as the 16 rows and up to 8 query heads
+// as the 8 columns, S^T = K q^T, then O^T = V^T P^T, so the tiles are A operands as they lie in
+// shared memory (ldmatrix, transposed for V) and an MMA is full for a group of 8. f32 pages
+// would lose precision there; they use packed f32 FMAs, a key's row split over a few lanes.
 #include <cuda_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
 
 #include "paged.hpp"
 #include "sx_device.cuh"
@@ -15,7 +37,9 @@
 namespace sx {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxSmem = 227 * 1024;
 
 struct AttnK {
   const uint8_t* q;
@@ -24,140 +48,940 @@ struct AttnK {
   const uint8_t *k, *v;
   const int *table, *lens;
   int* status;
+  uint8_t* ws;
   long long q_stride, out_stride;                    // elements
-  long long page_stride, head_stride, token_stride;  // elements
+  long long page_stride, head_stride, token_stride;  // bytes
   long long table_stride;
   int n, Hkv, G, H, page_shift, width, n_pages;
+  int stages;  // tiles in a warp's ring
+  int direct;  // 1: CTA c is (request c / Hkv, kv head c % Hkv); nothing is split over CTAs
   float scale;
 };
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+// Workspace: per CTA a record of the partial that begins in it, then two partials per CTA
+// (the one its share begins inside of, the one it ends inside of).
+struct Joint {
+  int i, h, pieces, pad;  // pieces: partials of (i, h), 0: none begins here
+};
+__host__ __device__ inline size_t ws_stats_off(int ctas) { return (size_t)ctas * sizeof(Joint); }
+__host__ __device__ inline size_t ws_o_off(int ctas, int G) { return ws_stats_off(ctas) + (size_t)2 * ctas * G * 8; }
+__host__ __device__ inline size_t ws_bytes(int ctas, int G, int hd) {
+  return ws_o_off(ctas, G) + (size_t)2 * ctas * G * hd * 4 + 16;
+}
+
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-template <int HD, typename QT, typename CT, int GM>
-__global__ void __launch_bounds__(kWarps * 32) k_paged_attention(const AttnK a) {
-  constexpr int E = HD / 32;
-  extern __shared__ __align__(16) float smem[];  // [kWarps][GM][HD + 2]
-  pdl_launch_dependents();
-  pdl_wait();
-  const int i = blockIdx.x / a.Hkv, h = blockIdx.x % a.Hkv;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int len = max(0, ld_cg(a.lens + i));
-  const long long cap = (long long)a.width << a.page_shift;
-  if (len > cap) {
-    len = (int)cap;
-    if (a.status && threadIdx.x == 0) *a.status = SX_E_RANGE;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// What a maximum of -inf (nothing seen, or only scores of -inf) is taken as.
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+
+// ---- 16-bit pages -----------------------------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
-  float q[GM][E], o[GM][E], m[GM], l[GM];
-  const QT* qp = reinterpret_cast<const QT*>(a.q) + (size_t)i * a.q_stride + (size_t)h * a.G * HD;
-#pragma unroll
-  for (int g = 0; g < GM; g++) {
-    m[g] = -INFINITY;
-    l[g] = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      q[g][e] = g < a.G ? to_f32(qp[(size_t)g * HD + lane + 32 * e]) : 0.f;
-      o[g][e] = 0.f;
-    }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack16(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  } else {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
-  const float sl2 = a.scale * 1.4426950408889634f;
-  for (int t = warp; t < len; t += kWarps) {
-    const int page = ld_cg(a.table + (size_t)i * a.table_stride + (t >> a.page_shift));
-    const bool there = (unsigned)page < (unsigned)a.n_pages;
-    if (!there && a.status && lane == 0) *a.status = SX_E_RANGE;
-    const size_t at = there ? (size_t)page * a.page_stride + (size_t)h * a.head_stride +
-                                  (size_t)(t & ((1 << a.page_shift) - 1)) * a.token_stride
-                            : 0;
-    float kv[E], vv[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      kv[e] = there ? to_f32(reinterpret_cast<const CT*>(a.k)[at + lane + 32 * e]) : 0.f;
-      vv[e] = there ? to_f32(reinterpret_cast<const CT*>(a.v)[at + lane + 32 * e]) : 0.f;
-    }
-#pragma unroll
-    for (int g = 0; g < GM; g++) {
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; e++) s = fmaf(q[g][e], kv[e], s);
-      s = warp_sum(s) * sl2;
-      const float top = fmaxf(m[g], s), ref = top == -INFINITY ? 0.f : top;
-      const float alpha = exp2f(m[g] - ref), p = exp2f(s - ref);
-      m[g] = top;
-      l[g] = fmaf(l[g], alpha, p);
-#pragma unroll
-      for (int e = 0; e < E; e++) o[g][e] = fmaf(p, vv[e], o[g][e] * alpha);
-    }
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  float* mine = smem + (size_t)warp * GM * (HD + 2);
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// v as NL values of type T that add up to it: each the rounding of what the ones before leave.
+template <typename T, int NL>
+__device__ __forceinline__ void split16(float lo, float hi, uint32_t (&w)[NL]) {
 #pragma unroll
-  for (int g = 0; g < GM; g++) {
-#pragma unroll
-    for (int e = 0; e < E; e++) mine[g * (HD + 2) + lane + 32 * e] = o[g][e];
-    if (lane == 0) {
-      mine[g * (HD + 2) + HD] = m[g];
-      mine[g * (HD + 2) + HD + 1] = l[g];
+  for (int x = 0; x < NL; x++) {
+    w[x] = pack16<T>(lo, hi);
+    if (x + 1 < NL) {
+      const float2 r = unpack16<T>(w[x]);
+      lo -= r.x;
+      hi -= r.y;
     }
-  }
-  __syncthreads();
-  for (int x = threadIdx.x; x < a.G * HD; x += kWarps * 32) {
-    const int g = x / HD, e = x % HD;
-    float top = -INFINITY;
-    for (int w = 0; w < kWarps; w++) top = fmaxf(top, smem[(w * GM + g) * (HD + 2) + HD]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc = 0.f;
-    for (int w = 0; w < kWarps; w++) {
-      const float* r = smem + (w * GM + g) * (HD + 2);
-      const float f = exp2f(r[HD] - ref);
-      sum = fmaf(r[HD + 1], f, sum);
-      acc = fmaf(r[e], f, acc);
-    }
-    const int head = h * a.G + g;
-    put(reinterpret_cast<QT*>(a.out) + (size_t)i * a.out_stride + (size_t)head * HD + e,
-        sum == 0.f ? 0.f : __fdiv_rn(acc, sum));
-    if (a.lse && e == 0)
-      a.lse[(size_t)i * a.H + head] = sum == 0.f ? -INFINITY : 0.6931471805599453f * (ref + log2f(sum));
   }
 }
 
-template <int HD, typename QT, typename CT, int GM>
-cudaError_t launch_g(const AttnK& a, cudaStream_t st) {
-  const size_t smem = (size_t)kWarps * GM * (HD + 2) * 4;
-  const cudaError_t e =
-      cudaFuncSetAttribute(k_paged_attention<HD, QT, CT, GM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+// The same for weights, which are not negative: every part but the last is cut off, not rounded,
+// and none that is left over is zero (2^-30 of the weight at least, 2^-22 in f16), so that an
+// infinite value times the parts is infinite and not inf - inf or 0 inf.
+template <typename T, int NP>
+__device__ __forceinline__ void split_weights(float lo, float hi, uint32_t (&w)[NP]) {
+  constexpr bool f16 = std::is_same<T, __half>::value;
+  const float least_lo = lo * (f16 ? 0x1p-22f : 0x1p-30f), least_hi = hi * (f16 ? 0x1p-22f : 0x1p-30f);
+#pragma unroll
+  for (int x = 0; x < NP; x++) {
+    if (x + 1 == NP) {
+      w[x] = pack16<T>(lo, hi);
+    } else {
+      if constexpr (f16)
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(w[x]) : "f"(hi), "f"(lo));
+      else
+        w[x] = __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+      const float2 r = unpack16<T>(w[x]);
+      lo = fmaxf(lo - r.x, least_lo);
+      hi = fmaxf(hi - r.y, least_hi);
+    }
+  }
+}
+
+// One warp's online softmax over tiles of 16-bit keys and values. Lane (g = lane / 4, t = lane % 4)
+// holds the scores of keys g and g + 8 of each 16 for heads 2t and 2t + 1 of each 8, and output
+// elements g and g + 8 of each 16 for the same heads.
+template <int HD_, typename QT_, typename CT_, int GM>
+struct Mma {
+  using QT = QT_;
+  using CT = CT_;
+  static constexpr int HD = HD_;
+  static constexpr int NW = HD == 256 ? 4 : 8;                   // warps per CTA
+  static constexpr int TK = HD == 32 ? 64 : HD == 64 ? 32 : 16;  // keys per tile
+  static constexpr int RB = HD * 2, CPR = RB / 16;
+  static constexpr int NT = (GM + 7) / 8, MT = TK / 16, KS = HD / 16;
+  static constexpr bool kF16 = std::is_same<CT, __half>::value;
+  static constexpr bool kQ32 = sizeof(QT) == 4;
+  // f32 queries and weights pass the tensor cores as sums of 16-bit values: three bf16 hold 24
+  // bits; two f16 hold 22, of values that are first scaled to the top of f16's range. 16-bit
+  // queries are exact; their weights keep 16 (bf16) or 22 (f16) bits, far below the rounding
+  // of the result, where a single value would add a rounding as large as the result's own.
+  static constexpr int NL = kQ32 ? (kF16 ? 2 : 3) : 1;
+  static constexpr int NP = kQ32 ? (kF16 ? 2 : 3) : 2;
+  // f16 weights are kept as 2^10 p, so that their low parts stay above f16's smallest step
+  static constexpr float kLift = kF16 ? 10.f : 0.f;
+
+  uint32_t q[NT][NL][KS][2];
+  float o[NT][KS][4];
+  float m[NT][2], l[NT][2], sl2[NT][2];
+
+  static __device__ __forceinline__ uint32_t at(int row, int chunk) {  // byte of a 16-byte chunk in a tile
+    if constexpr (CPR == 4) return row * RB + ((chunk ^ ((row >> 1) & 3)) << 4);
+    return row * RB + ((chunk ^ (row & 7)) << 4);
+  }
+
+  __device__ __forceinline__ void start(const AttnK& a, int i, int h, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    const QT* qp = reinterpret_cast<const QT*>(a.q) + (size_t)i * a.q_stride + (size_t)h * a.G * HD;
+    const float base = a.scale * kLog2e;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int head = nt * 8 + g;
+      const bool on = head < a.G;
+      float up = 1.f, down = 1.f;  // powers of two
+      if constexpr (kQ32) {
+        float2 x[KS][2];
+        float top = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            x[ks][c] = on ? __ldcg(reinterpret_cast<const float2*>(qp + (size_t)head * HD + ks * 16 + c * 8 + 2 * t))
+                          : make_float2(0.f, 0.f);
+            top = fmaxf(top, fmaxf(fabsf(x[ks][c].x), fabsf(x[ks][c].y)));
+          }
+        if constexpr (kF16) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          if (top > 0.f && top < INFINITY) {
+            const int ex = min(max(ilogbf(top), -100), 127) - 10;  // the head's largest lands in [2^10, 2^11)
+            up = ldexpf(1.f, -ex);
+            down = ldexpf(1.f, ex);
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            uint32_t w[NL];
+            split16<CT, NL>(x[ks][c].x * up, x[ks][c].y * up, w);
+#pragma unroll
+            for (int y = 0; y < NL; y++) q[nt][y][ks][c] = w[y];
+          }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+          for (int c = 0; c < 2; c++)
+            q[nt][0][ks][c] =
+                on ? __ldcg(reinterpret_cast<const uint32_t*>(qp + (size_t)head * HD + ks * 16 + c * 8 + 2 * t)) : 0u;
+      }
+      const float mine = base * down;
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        sl2[nt][c] = __shfl_sync(0xffffffffu, mine, 4 * (2 * t + c));
+        m[nt][c] = -INFINITY;
+        l[nt][c] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < KS; j++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[nt][j][c] = 0.f;
+    }
+  }
+
+  // `valid` of the tile's keys count; the others' rows are zeros.
+  __device__ __forceinline__ void tile(uint32_t ks_, uint32_t vs_, int valid, int lane) {
+    const int g = lane >> 2;
+    const int r16 = lane & 15, c1 = lane >> 4;  // ldmatrix: row and half chunk of this lane's address
+    float s[MT][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+      float low[NT][4];  // the products of a split query's lower parts
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) s[mt][nt][c] = low[nt][c] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        uint32_t a[4];
+        ldsm4(a, ks_ + at(mt * 16 + r16, 2 * ks + c1));
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int y = 0; y < NL; y++) mma16816<CT>(y ? low[nt] : s[mt][nt], a, q[nt][y][ks][0], q[nt][y][ks][1]);
+      }
+      if constexpr (NL > 1) {
+        // an infinite key makes the lower parts' products infinite too, of either sign
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int c = 0; c < 4; c++) s[mt][nt][c] = isinf(s[mt][nt][c]) ? s[mt][nt][c] : s[mt][nt][c] + low[nt][c];
+      }
+    }
+    uint32_t p[MT][NT][NP][2];
+    bool turned = false;
+    float alpha[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          s[mt][nt][c] = mt * 16 + g + (c >> 1) * 8 < valid ? s[mt][nt][c] * sl2[nt][c & 1] : -INFINITY;
+          top[c & 1] = fmaxf(top[c & 1], s[mt][nt][c]);
+        }
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], off));
+        top[c] = fmaxf(top[c], m[nt][c]);
+        const float ref = finite_or_zero(top[c]);
+        alpha[nt][c] = exp2f(m[nt][c] - ref);
+        turned |= alpha[nt][c] != 1.f;
+        m[nt][c] = top[c];
+        top[c] = ref - kLift;
+        l[nt][c] *= alpha[nt][c];
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          s[mt][nt][c] = exp2f(s[mt][nt][c] - top[c & 1]);
+          l[nt][c & 1] += s[mt][nt][c];
+        }
+        uint32_t lo[NP], hi[NP];
+        split_weights<CT, NP>(s[mt][nt][0], s[mt][nt][1], lo);
+        split_weights<CT, NP>(s[mt][nt][2], s[mt][nt][3], hi);
+#pragma unroll
+        for (int y = 0; y < NP; y++) {
+          p[mt][nt][y][0] = transpose8x8(lo[y]);
+          p[mt][nt][y][1] = transpose8x8(hi[y]);
+        }
+      }
+    }
+    if (__any_sync(0xffffffffu, turned)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int j = 0; j < KS; j++)
+#pragma unroll
+          for (int c = 0; c < 4; c++) o[nt][j][c] *= alpha[nt][c & 1];
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+      for (int j = 0; j < KS; j++) {
+        uint32_t a[4];
+        // rows: keys (lane & 7) + 8 (lane / 16); chunks: elements 16 j + 8 ((lane / 8) & 1)
+        ldsm4_t(a, vs_ + at(mt * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * j + ((lane >> 3) & 1)));
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int y = 0; y < NP; y++) mma16816<CT>(o[nt][j], a, p[mt][nt][y][0], p[mt][nt][y][1]);
+      }
+  }
+
+  // f(head, element, value of o, l) for every output of the group this lane holds, then
+  // w(head, m, l) by one lane per head; m and l over all keys the warp has seen.
+  template <class F, class W>
+  __device__ __forceinline__ void finish(int G, int lane, F&& f, W&& w) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        float sum = l[nt][c];
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        const int head = nt * 8 + 2 * t + c;
+        if (head < G) {
+#pragma unroll
+          for (int j = 0; j < KS; j++) {
+            f(head, j * 16 + g, o[nt][j][c], sum);
+            f(head, j * 16 + g + 8, o[nt][j][c + 2], sum);
+          }
+          if (g == 0) w(head, m[nt][c], sum);
+        }
+      }
+  }
+};
+
+// ---- f32 pages --------------------------------------------------------------------------
+
+// Sums over LPK neighbouring lanes of each of V values, left with every lane: halves of the
+// values are exchanged while there are several (each lane adds up its own share), then gathered
+// back in the opposite order.
+template <int V, int MASK>
+__device__ __forceinline__ void sum_over(float* a, int lane) {
+  if constexpr (MASK > 0) {
+    if constexpr (V > 1) {
+      constexpr int HV = V / 2;
+      const bool up = lane & MASK;
+      float keep[HV];
+#pragma unroll
+      for (int i = 0; i < HV; i++) {
+        const float send = up ? a[i] : a[i + HV];
+        keep[i] = (up ? a[i + HV] : a[i]) + __shfl_xor_sync(0xffffffffu, send, MASK);
+      }
+      sum_over<HV, MASK / 2>(keep, lane);
+#pragma unroll
+      for (int i = 0; i < HV; i++) {
+        const float other = __shfl_xor_sync(0xffffffffu, keep[i], MASK);
+        a[i] = up ? other : keep[i];
+        a[i + HV] = up ? keep[i] : other;
+      }
+    } else {
+      a[0] += __shfl_xor_sync(0xffffffffu, a[0], MASK);
+      sum_over<1, MASK / 2>(a, lane);
+    }
+  }
+}
+
+// One warp's online softmax over tiles of f32 keys and values on the FMA pipes. LPK lanes share
+// a key, each E = HD / LPK of its elements (16-byte chunks LPK apart); the 32 / LPK lane groups
+// take keys in turn, each with a running maximum of its own, and are joined at the end.
+template <int HD_, int GM>
+struct Fma {
+  using QT = float;
+  using CT = float;
+  static constexpr int HD = HD_;
+  static constexpr int NW = 8;
+  static constexpr int TK = 1024 / HD;  // keys per tile: 8 KB of keys and values
+  static constexpr int RB = HD * 4, CPR = RB / 16;
+  // at most 64 query elements and 64 output elements a lane
+  static constexpr int LPK0 = GM * HD / 64 < 4 ? 4 : GM * HD / 64;
+  static constexpr int LPK = LPK0 < HD / 16 ? HD / 16 : LPK0;
+  static constexpr int E = HD / LPK, KG = 32 / LPK;
+  static constexpr int NK = TK / KG;           // keys of a tile per lane group
+  static constexpr int KB = GM == 16 || NK < 4 ? 2 : 4;  // keys folded at a time
+  static constexpr float kLift = 0.f;
+  static_assert(LPK <= 32 && E >= 4 && TK % KG == 0 && NK % KB == 0, "lane split");
+
+  unsigned long long q[GM][E / 2], o[GM][E / 2];
+  float m[GM], l[GM], sl2;
+
+  static __device__ __forceinline__ uint32_t at(int row, int chunk) {
+    if constexpr (LPK == 4) return row * RB + ((chunk ^ ((row & 1) << 2)) << 4);
+    return row * RB + (chunk << 4);
+  }
+
+  __device__ __forceinline__ void start(const AttnK& a, int i, int h, int lane) {
+    const int hs = lane % LPK;
+    const float* qp = reinterpret_cast<const float*>(a.q) + (size_t)i * a.q_stride + (size_t)h * a.G * HD;
+    sl2 = a.scale * kLog2e;
+#pragma unroll
+    for (int g = 0; g < GM; g++) {
+#pragma unroll
+      for (int j = 0; j < E / 4; j++) {
+        const float4 x = g < a.G ? __ldcg(reinterpret_cast<const float4*>(qp + (size_t)g * HD) + hs + LPK * j)
+                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+        q[g][2 * j] = pack2(x.x, x.y);
+        q[g][2 * j + 1] = pack2(x.z, x.w);
+      }
+#pragma unroll
+      for (int e = 0; e < E / 2; e++) o[g][e] = 0ull;
+      m[g] = -INFINITY;
+      l[g] = 0.f;
+    }
+  }
+
+  static __device__ __forceinline__ void row(uint32_t addr, int r, int hs, unsigned long long (&x)[E / 2]) {
+#pragma unroll
+    for (int j = 0; j < E / 4; j++)
+      asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];"
+                   : "=l"(x[2 * j]), "=l"(x[2 * j + 1])
+                   : "r"(addr + at(r, hs + LPK * j))
+                   : "memory");
+  }
+
+  __device__ __forceinline__ void tile(uint32_t ks_, uint32_t vs_, int valid, int lane) {
+    const int hs = lane % LPK, kg = lane / LPK;
+#pragma unroll
+    for (int b = 0; b < NK / KB; b++) {
+      float s[GM * KB];
+#pragma unroll
+      for (int kk = 0; kk < KB; kk++) {
+        unsigned long long x[E / 2];
+        row(ks_, kg + KG * (b * KB + kk), hs, x);
+#pragma unroll
+        for (int g = 0; g < GM; g++) {
+          unsigned long long d = mul2(q[g][0], x[0]);
+#pragma unroll
+          for (int e = 1; e < E / 2; e++) d = fma2(q[g][e], x[e], d);
+          float lo, hi;
+          unpack2(d, lo, hi);
+          s[g * KB + kk] = lo + hi;
+        }
+      }
+      sum_over<GM * KB, LPK / 2>(s, lane);
+      bool turned = false;
+      float alpha[GM];
+#pragma unroll
+      for (int g = 0; g < GM; g++) {
+        float top = m[g];
+#pragma unroll
+        for (int kk = 0; kk < KB; kk++) {
+          s[g * KB + kk] = kg + KG * (b * KB + kk) < valid ? s[g * KB + kk] * sl2 : -INFINITY;
+          top = fmaxf(top, s[g * KB + kk]);
+        }
+        const float ref = finite_or_zero(top);
+        alpha[g] = exp2f(m[g] - ref);
+        turned |= alpha[g] != 1.f;
+        m[g] = top;
+        l[g] *= alpha[g];
+#pragma unroll
+        for (int kk = 0; kk < KB; kk++) {
+          s[g * KB + kk] = exp2f(s[g * KB + kk] - ref);
+          l[g] += s[g * KB + kk];
+        }
+      }
+      if (__any_sync(0xffffffffu, turned)) {
+#pragma unroll
+        for (int g = 0; g < GM; g++) {
+          const unsigned long long f = pack2(alpha[g], alpha[g]);
+#pragma unroll
+          for (int e = 0; e < E / 2; e++) o[g][e] = mul2(o[g][e], f);
+        }
+      }
+#pragma unroll
+      for (int kk = 0; kk < KB; kk++) {
+        unsigned long long x[E / 2];
+        row(vs_, kg + KG * (b * KB + kk), hs, x);
+#pragma unroll
+        for (int g = 0; g < GM; g++) {
+          const unsigned long long f = pack2(s[g * KB + kk], s[g * KB + kk]);
+#pragma unroll
+          for (int e = 0; e < E / 2; e++) o[g][e] = fma2(f, x[e], o[g][e]);
+        }
+      }
+    }
+  }
+
+  template <class F, class W>
+  __device__ __forceinline__ void finish(int G, int lane, F&& f, W&& w) {
+    const int hs = lane % LPK, kg = lane / LPK;
+#pragma unroll
+    for (int g = 0; g < GM; g++) {
+      float top = m[g];
+#pragma unroll
+      for (int off = LPK; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      const float fac = exp2f(m[g] - finite_or_zero(top));
+      float sum = l[g] * fac;
+#pragma unroll
+      for (int off = LPK; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+      float x[E];
+#pragma unroll
+      for (int e = 0; e < E / 2; e++) unpack2(o[g][e], x[2 * e], x[2 * e + 1]);
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        x[e] *= fac;
+#pragma unroll
+        for (int off = LPK; off < 32; off <<= 1) x[e] += __shfl_xor_sync(0xffffffffu, x[e], off);
+      }
+      if (g < G && g % KG == kg) {
+#pragma unroll
+        for (int e = 0; e < E; e++) f(g, (hs + LPK * (e / 4)) * 4 + e % 4, x[e], sum);
+        if (hs == 0) w(g, top, sum);
+      }
+    }
+  }
+};
+
+// ---- the walk over the tiles --------------------------------------------------------------
+
+// A place in the line of tiles: tile t of kv head h of request i. Lane-parallel: every lane of
+// the warp holds the same place, and the lengths of 32 requests are kept one per lane.
+template <int TK>
+struct Place {
+  int i, h, t, len, tiles;
+  int base, cached;  // lens[base + lane]
+
+  __device__ __forceinline__ void at_request(const AttnK& a, int cap, int req, int lane) {
+    if (req < base || req >= base + 32) {
+      base = req;
+      cached = req + lane < a.n ? min(max(ld_cg(a.lens + req + lane), 0), cap) : 0;
+    }
+    i = req;
+    len = __shfl_sync(0xffffffffu, cached, req - base);
+    tiles = (len + TK - 1) / TK;
+  }
+  __device__ __forceinline__ void next(const AttnK& a, int cap, int lane) {
+    if (++t < tiles) return;
+    t = 0;
+    if (++h < a.Hkv) return;
+    h = 0;
+    do {
+      at_request(a, cap, i + 1, lane);
+    } while (len == 0 && i + 1 < a.n);
+  }
+};
+
+struct Piece {
+  int i, h;
+  int valid, begins, ends, rest;  // rest: tiles of (i, h) behind this piece
+};
+
+template <class M>
+struct Smem {
+  static constexpr int NT = M::NW * 32;
+  long long before[NT + 1];  // tiles of the requests before thread t's strip
+  long long part[33];
+  Piece piece[2 * M::NW];
+  float ml[2 * M::NW][16][2];
+};
+
+template <class M>
+__global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a) {
+  constexpr int NW = M::NW, NT = NW * 32, TK = M::TK, HD = M::HD, RB = M::RB, CPR = M::CPR;
+  constexpr int TILE = 2 * TK * RB;
+  using QT = typename M::QT;
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ Smem<M> sm;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = blockIdx.x, ctas = gridDim.x;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  const int cap = (int)min((long long)a.width << a.page_shift, 0x7fffffffll);
+  Place<TK> pc;
+  pc.base = -64;
+  pc.cached = 0;
+  pc.h = pc.t = 0;
+  long long todo;      // tiles of this warp
+  long long share = 0; // tiles per CTA
+  if (tid < 2 * NW) sm.piece[tid].valid = 0;
+
+  if (a.direct) {
+    pc.at_request(a, cap, cta / a.Hkv, lane);
+    pc.h = cta % a.Hkv;
+    const int w0 = (int)((long long)pc.tiles * warp / NW), w1 = (int)((long long)pc.tiles * (warp + 1) / NW);
+    pc.t = w0;
+    todo = w1 - w0;
+  } else {
+    // tiles before each strip of requests (a strip per thread) and in all
+    const int strip = (a.n + NT - 1) / NT;
+    long long mine = 0;
+    for (int i = min(a.n, tid * strip); i < min(a.n, (tid + 1) * strip); i++)
+      mine += (long long)((min(max(ld_cg(a.lens + i), 0), cap) + TK - 1) / TK) * a.Hkv;
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (lane == 31) sm.part[warp] = inc;
+    __syncthreads();
+    long long base = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      if (w < warp) base += sm.part[w];
+      total += sm.part[w];
+    }
+    sm.before[tid] = base + inc - mine;
+    if (tid == 0) sm.before[NT] = total;
+    __syncthreads();
+    share = max((total + ctas - 1) / ctas, (long long)NW);
+    const long long c0 = min(total, share * cta), c1 = min(total, c0 + share);
+    const long long w0 = c0 + (c1 - c0) * warp / NW, w1 = c0 + (c1 - c0) * (warp + 1) / NW;
+    todo = w1 - w0;
+    if (todo > 0) {
+      // the strip, then the request, that holds tile w0
+      int st = 0;
+#pragma unroll
+      for (int x = 0; x < NT / 32; x++) {
+        const int c = x * 32 + lane;
+        const unsigned hit = __ballot_sync(0xffffffffu, sm.before[c] <= w0 && w0 < sm.before[c + 1]);
+        if (hit) st = x * 32 + __ffs(hit) - 1;
+      }
+      long long off = w0 - sm.before[st];
+      int i = st * strip;
+      for (;; i += 32) {
+        const int len = i + lane < a.n ? min(max(ld_cg(a.lens + i + lane), 0), cap) : 0;
+        long long run = (long long)((len + TK - 1) / TK) * a.Hkv;
+        const long long own = run;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long u = __shfl_up_sync(0xffffffffu, run, o);
+          if (lane >= o) run += u;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, run > off);
+        if (hit) {
+          const int who = __ffs(hit) - 1;
+          off -= __shfl_sync(0xffffffffu, run - own, who);
+          i += who;
+          break;
+        }
+        off -= __shfl_sync(0xffffffffu, run, 31);
+        if (i + 32 >= a.n) break;  // not reached: before[] holds the tile
+      }
+      pc.at_request(a, cap, i, lane);
+      pc.h = (int)(off / pc.tiles);
+      pc.t = (int)(off % pc.tiles);
+    }
+  }
+
+  // requests without keys, and lengths that do not fit
+  for (long long i0 = cta; i0 < a.n; i0 += (long long)ctas * NT) {
+    const long long i = i0 + (long long)ctas * tid;
+    const int len = i < a.n ? ld_cg(a.lens + i) : 1;
+    if (i < a.n && len > cap && a.status) *a.status = SX_E_RANGE;
+    unsigned none = __ballot_sync(0xffffffffu, i < a.n && len <= 0);
+    while (none) {
+      const int who = __ffs(none) - 1;
+      none &= none - 1;
+      const long long j = __shfl_sync(0xffffffffu, i, who);
+      QT* out = reinterpret_cast<QT*>(a.out) + j * a.out_stride;
+      for (int x = lane; x < a.H * HD; x += 32) put(out + x, 0.f);
+      if (a.lse)
+        for (int x = lane; x < a.H; x += 32) a.lse[j * a.H + x] = -INFINITY;
+    }
+  }
+  __syncthreads();  // sm.piece is cleared
+
+  uint8_t* ring = dyn + (size_t)warp * a.stages * TILE;
+  const uint32_t ring_s = smem_addr(ring);
+  // Where a partial at the start of a run goes. Warp 0's is the share's own first partial.
+  Joint* joint = reinterpret_cast<Joint*>(a.ws);
+  float* ws_ml = reinterpret_cast<float*>(a.ws + ws_stats_off(ctas));
+  float* ws_o = reinterpret_cast<float*>(a.ws + ws_o_off(ctas, a.G));
+  float* first_o = reinterpret_cast<float*>(dyn + (size_t)NW * a.stages * TILE);  // [NW - 1][G][HD]
+
+  // the copying side runs ahead of the computing side by the ring's depth
+  Place<TK> pp = pc;
+  long long to_copy = todo;
+  int page_of = -1, page_base = 0, pages = 0;  // request and first of the 32 pages held one per lane
+  const int page_mask = (1 << a.page_shift) - 1;
+  auto copy_next = [&](int stage) {
+    if (to_copy > 0) {
+      const int key0 = pp.t * TK, p0 = key0 >> a.page_shift;
+      if (page_of != pp.i || p0 >= page_base + 32 || p0 < page_base) {
+        page_of = pp.i;
+        page_base = p0 & ~31;
+        const int idx = page_base + lane;
+        int page = -1;
+        if (idx <= (pp.len - 1) >> a.page_shift) {
+          page = ld_cg(a.table + (size_t)pp.i * a.table_stride + idx);
+          if ((unsigned)page >= (unsigned)a.n_pages) {
+            page = -1;
+            if (a.status) *a.status = SX_E_RANGE;
+          }
+        }
+        pages = page;
+      }
+      const uint32_t dst = ring_s + stage * TILE;
+      const size_t head = (size_t)pp.h * a.head_stride;
+#pragma unroll
+      for (int x = 0; x < TK * CPR / 32; x++) {
+        const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR;
+        const int key = key0 + r;
+        const int page = __shfl_sync(0xffffffffu, pages, (key >> a.page_shift) - page_base);
+        const bool there = key < pp.len && page >= 0;
+        const size_t off = there ? (size_t)page * a.page_stride + head + (size_t)(key & page_mask) * a.token_stride + c * 16
+                                 : 0;
+        const uint32_t d = dst + M::at(r, c);
+        cp_async16(d, a.k + off, there ? 16 : 0);
+        cp_async16(d + TK * RB, a.v + off, there ? 16 : 0);
+      }
+      to_copy--;
+      if (to_copy > 0) pp.next(a, cap, lane);
+    }
+    cp_commit();
+  };
+  int into = 0, from = 0;
+  for (int x = 0; x < a.stages - 1; x++) {
+    copy_next(into);
+    into = into + 1 == a.stages ? 0 : into + 1;
+  }
+
+  M mine;
+  bool fresh = true, began = false;
+  for (; todo > 0; todo--) {
+    copy_next(into);
+    into = into + 1 == a.stages ? 0 : into + 1;
+    if (fresh) {
+      mine.start(a, pc.i, pc.h, lane);
+      began = pc.t == 0;
+      fresh = false;
+    }
+    if (a.stages == 3)
+      cp_wait<2>();
+    else if (a.stages == 2)
+      cp_wait<1>();
+    else
+      cp_wait<3>();
+    __syncwarp();
+    const uint32_t tile = ring_s + from * TILE;
+    mine.tile(tile, tile + TK * RB, min(TK, pc.len - pc.t * TK), lane);
+    from = from + 1 == a.stages ? 0 : from + 1;
+    __syncwarp();  // every lane has read the tile before it is overwritten
+    const bool ends = pc.t + 1 == pc.tiles;
+    if (ends || todo == 1) {
+      if (ends && began) {
+        QT* out = reinterpret_cast<QT*>(a.out) + (size_t)pc.i * a.out_stride + (size_t)pc.h * a.G * HD;
+        float* lse = a.lse ? a.lse + (size_t)pc.i * a.H + (size_t)pc.h * a.G : nullptr;
+        mine.finish(
+            a.G, lane,
+            [&](int head, int d, float v, float sum) { put(out + head * HD + d, sum == 0.f ? 0.f : __fdiv_rn(v, sum)); },
+            [&](int head, float top, float sum) {
+              if (lse) lse[head] = sum == 0.f ? -INFINITY : kLn2 * (finite_or_zero(top) + log2f(sum) - M::kLift);
+            });
+      } else {
+        // a partial: the run's last one may lie in the ring, which is then done with
+        const int slot = 2 * warp + (todo == 1);
+        const bool out_of_cta = warp == 0 && todo > 1;
+        float* dst = todo == 1    ? reinterpret_cast<float*>(ring)
+                     : out_of_cta ? ws_o + (size_t)2 * cta * a.G * HD
+                                  : first_o + (size_t)(warp - 1) * a.G * HD;
+        float* ml = out_of_cta ? ws_ml + (size_t)2 * cta * a.G * 2 : &sm.ml[slot][0][0];
+        mine.finish(
+            a.G, lane, [&](int head, int d, float v, float) { dst[head * HD + d] = v; },
+            [&](int head, float top, float sum) {
+              ml[2 * head] = top;
+              ml[2 * head + 1] = sum;
+            });
+        if (lane == 0 && !out_of_cta) {
+          Piece& p = sm.piece[slot];
+          p.i = pc.i;
+          p.h = pc.h;
+          p.begins = began;
+          p.ends = ends;
+          p.rest = pc.tiles - pc.t - 1;
+          p.valid = 1;
+        }
+      }
+      fresh = true;
+    }
+    if (todo > 1) pc.next(a, cap, lane);
+  }
+  cp_wait<0>();
+  __syncthreads();
+
+  // join the warps' partials, in key order
+  auto piece_o = [&](int x) {
+    return (x & 1) ? reinterpret_cast<const float*>(dyn + (size_t)(x >> 1) * a.stages * TILE)
+                   : first_o + (size_t)((x >> 1) - 1) * a.G * HD;
+  };
+  bool leaves = false;
+  for (int x = 0; x < 2 * NW;) {
+    const Piece first = sm.piece[x];
+    if (!first.valid) {
+      x++;
+      continue;
+    }
+    int last = x;
+    for (int y = x + 1; y < 2 * NW; y++) {
+      const Piece& p = sm.piece[y];
+      if (!p.valid) continue;
+      if (p.i != first.i || p.h != first.h) break;
+      last = y;
+    }
+    const Piece end = sm.piece[last];
+    const bool whole = first.begins && end.ends;
+    const int slot = 2 * cta + (first.begins ? 1 : 0);
+    for (int e = tid; e < a.G * HD; e += NT) {
+      const int head = e / HD, d = e % HD;
+      float top = -INFINITY;
+      for (int y = x; y <= last; y++)
+        if (sm.piece[y].valid) top = fmaxf(top, sm.ml[y][head][0]);
+      const float ref = finite_or_zero(top);
+      float sum = 0.f, v = 0.f;
+      for (int y = x; y <= last; y++)
+        if (sm.piece[y].valid) {
+          const float f = exp2f(sm.ml[y][head][0] - ref);
+          sum = fmaf(sm.ml[y][head][1], f, sum);
+          v = fmaf(piece_o(y)[e], f, v);
+        }
+      if (whole) {
+        put(reinterpret_cast<QT*>(a.out) + (size_t)first.i * a.out_stride + (size_t)first.h * a.G * HD + e,
+            sum == 0.f ? 0.f : __fdiv_rn(v, sum));
+        if (a.lse && d == 0)
+          a.lse[(size_t)first.i * a.H + (size_t)first.h * a.G + head] =
+              sum == 0.f ? -INFINITY : kLn2 * (ref + log2f(sum) - M::kLift);
+      } else {
+        ws_o[(size_t)slot * a.G * HD + e] = v;
+        if (d == 0) {
+          ws_ml[((size_t)slot * a.G + head) * 2] = top;
+          ws_ml[((size_t)slot * a.G + head) * 2 + 1] = sum;
+        }
+      }
+    }
+    if (!whole && first.begins) {
+      leaves = true;
+      if (tid == 0) {
+        Joint j;
+        j.i = first.i;
+        j.h = first.h;
+        j.pieces = 1 + (int)((end.rest + share - 1) / share);
+        j.pad = 0;
+        joint[cta] = j;
+      }
+    }
+    x = last + 1;
+  }
+  if (!a.direct && !leaves && tid == 0) joint[cta] = Joint{0, 0, 0, 0};
+}
+
+// Joins the partials of one query head of the (request, kv head) that begins in CTA blockIdx.x's
+// share and goes on behind it: the CTA's second partial, then the first ones of the CTAs after it.
+template <int HD, typename QT>
+__global__ void __launch_bounds__(HD < 128 ? 128 : HD) k_paged_join(const AttnK a, int ctas, float lift) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int cta = blockIdx.x, head = blockIdx.y;
+  const int4 raw = __ldcg(reinterpret_cast<const int4*>(a.ws) + cta);
+  const int pieces = raw.z;
+  if (pieces == 0) return;
+  const float* ml = reinterpret_cast<const float*>(a.ws + ws_stats_off(ctas));
+  const float* o = reinterpret_cast<const float*>(a.ws + ws_o_off(ctas, a.G));
+  auto slot = [&](int y) { return (size_t)(y == 0 ? 2 * cta + 1 : 2 * (cta + y)) * a.G + head; };
+  const int d = threadIdx.x;
+  if (d >= HD) return;
+  float top = -INFINITY;
+  for (int y = 0; y < pieces; y++) top = fmaxf(top, __ldcg(ml + slot(y) * 2));
+  const float ref = finite_or_zero(top);
+  float sum = 0.f, v = 0.f;
+#pragma unroll 8
+  for (int y = 0; y < pieces; y++) {
+    const float2 s = __ldcg(reinterpret_cast<const float2*>(ml + slot(y) * 2));
+    const float f = exp2f(s.x - ref);
+    sum = fmaf(s.y, f, sum);
+    v = fmaf(__ldcg(o + slot(y) * HD + d), f, v);
+  }
+  const size_t row = (size_t)raw.y * a.G + head;
+  put(reinterpret_cast<QT*>(a.out) + (size_t)raw.x * a.out_stride + row * HD + d, sum == 0.f ? 0.f : __fdiv_rn(v, sum));
+  if (a.lse && d == 0) a.lse[(size_t)raw.x * a.H + row] = sum == 0.f ? -INFINITY : kLn2 * (ref + log2f(sum) - lift);
+}
+
+// Lengths up to this many keys are not split over CTAs.
+constexpr int kDirectLen = 512;
+
+template <class M>
+cudaError_t launch_m(AttnK a, long long bound, int sms, cudaStream_t st) {
+  constexpr int TILE = 2 * M::TK * M::RB;
+  const int partials = (M::NW - 1) * a.G * M::HD * 4;
+  a.stages = std::min(3, (kMaxSmem - (int)sizeof(Smem<M>) - 128 - partials) / (M::NW * TILE));
+  a.direct = bound <= kDirectLen;
+  const size_t smem = (size_t)M::NW * a.stages * TILE + partials;
+  cudaError_t e = cudaFuncSetAttribute(k_paged_attention<M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
+  const int grid = a.direct ? a.n * a.Hkv : sms;
   cudaLaunchAttribute attr[1];
-  cudaLaunchConfig_t cfg = launch_cfg(dim3(a.n * a.Hkv), dim3(kWarps * 32), smem, st, attr);
-  return cudaLaunchKernelEx(&cfg, k_paged_attention<HD, QT, CT, GM>, a);
+  cudaLaunchConfig_t cfg = launch_cfg(dim3(grid), dim3(M::NW * 32), smem, st, attr);
+  e = cudaLaunchKernelEx(&cfg, k_paged_attention<M>, a);
+  if (e != cudaSuccess || a.direct) return e;
+  cfg = launch_cfg(dim3(sms, a.G), dim3(M::HD < 128 ? 128 : M::HD), 0, st, attr);
+  return cudaLaunchKernelEx(&cfg, k_paged_join<M::HD, typename M::QT>, a, sms, M::kLift);
 }
 
 template <int HD, typename QT, typename CT>
-cudaError_t launch_t(const AttnK& a, cudaStream_t st) {
-  if (a.G <= 4) return launch_g<HD, QT, CT, 4>(a, st);
-  if (a.G <= 8) return launch_g<HD, QT, CT, 8>(a, st);
-  if constexpr (HD < 256) return launch_g<HD, QT, CT, 16>(a, st);
+cudaError_t launch_hd(const AttnK& a, long long bound, int sms, cudaStream_t st) {
+  if constexpr (sizeof(CT) == 4) {
+    if (a.G <= 2) return launch_m<Fma<HD, 2>>(a, bound, sms, st);
+    if (a.G <= 4) return launch_m<Fma<HD, 4>>(a, bound, sms, st);
+    if (a.G <= 8) return launch_m<Fma<HD, 8>>(a, bound, sms, st);
+    if constexpr (HD < 256) return launch_m<Fma<HD, 16>>(a, bound, sms, st);
+  } else {
+    if (a.G <= 8) return launch_m<Mma<HD, QT, CT, 8>>(a, bound, sms, st);
+    if constexpr (HD < 256) return launch_m<Mma<HD, QT, CT, 16>>(a, bound, sms, st);
+  }
   return cudaErrorInvalidValue;
 }
 
 template <typename QT, typename CT>
-cudaError_t launch_hd(const AttnK& a, int hd, cudaStream_t st) {
+cudaError_t launch_t(const AttnK& a, int hd, long long bound, int sms, cudaStream_t st) {
   switch (hd) {
-    case 32: return launch_t<32, QT, CT>(a, st);
-    case 64: return launch_t<64, QT, CT>(a, st);
-    case 128: return launch_t<128, QT, CT>(a, st);
-    default: return launch_t<256, QT, CT>(a, st);
+    case 32: return launch_hd<32, QT, CT>(a, bound, sms, st);
+    case 64: return launch_hd<64, QT, CT>(a, bound, sms, st);
+    case 128: return launch_hd<128, QT, CT>(a, bound, sms, st);
+    default: return launch_hd<256, QT, CT>(a, bound, sms, st);
   }
 }
 
 }  // namespace
 
-size_t paged_attention_workspace(int, int, int) { return 256; }
+size_t paged_attention_workspace(int G, int hd, int sms) { return ws_bytes(sms, G, hd); }
 
-cudaError_t launch_paged_attention(const sx_paged_attention_args& a, int, cudaStream_t st) {
+cudaError_t launch_paged_attention(const sx_paged_attention_args& a, int sms, cudaStream_t st) {
   AttnK k;
+  const long long ce = a.cache.dtype == SX_DTYPE_F32 ? 4 : 2;
   k.q = static_cast<const uint8_t*>(a.q);
   k.out = static_cast<uint8_t*>(a.out);
   k.lse = a.lse;
@@ -166,11 +990,12 @@ cudaError_t launch_paged_attention(const sx_paged_attention_args& a, int, cudaSt
   k.table = a.table;
   k.lens = a.lens;
   k.status = a.status;
+  k.ws = static_cast<uint8_t*>(a.workspace);
   k.q_stride = a.q_stride;
   k.out_stride = a.out_stride;
-  k.page_stride = a.cache.page_stride;
-  k.head_stride = a.cache.head_stride;
-  k.token_stride = a.cache.token_stride;
+  k.page_stride = a.cache.page_stride * ce;
+  k.head_stride = a.cache.head_stride * ce;
+  k.token_stride = a.cache.token_stride * ce;
   k.table_stride = a.table_stride;
   k.n = a.n_req;
   k.Hkv = a.cache.n_kv_heads;
@@ -179,14 +1004,20 @@ cudaError_t launch_paged_attention(const sx_paged_attention_args& a, int, cudaSt
   k.page_shift = __builtin_ctz((unsigned)a.cache.page_size);
   k.width = a.table_width;
   k.n_pages = a.cache.n_pages;
+  k.stages = 0;
+  k.direct = 0;
   k.scale = a.scale;
+  long long bound = (long long)a.table_width * a.cache.page_size;
+  if (a.max_len > 0) bound = std::min(bound, (long long)a.max_len);
   const int hd = a.cache.head_dim;
   const bool qf = a.q_dtype == SX_DTYPE_F32;
   switch (a.cache.dtype) {
-    case SX_DTYPE_F32: return launch_hd<float, float>(k, hd, st);
+    case SX_DTYPE_F32: return launch_t<float, float>(k, hd, bound, sms, st);
     case SX_DTYPE_BF16:
-      return qf ? launch_hd<float, __nv_bfloat16>(k, hd, st) : launch_hd<__nv_bfloat16, __nv_bfloat16>(k, hd, st);
-    default: return qf ? launch_hd<float, __half>(k, hd, st) : launch_hd<__half, __half>(k, hd, st);
+      return qf ? launch_t<float, __nv_bfloat16>(k, hd, bound, sms, st)
+                : launch_t<__nv_bfloat16, __nv_bfloat16>(k, hd, bound, sms, st);
+    default:
+      return qf ? launch_t<float, __half>(k, hd, bound, sms, st) : launch_t<__half, __half>(k, hd, bound, sms, st);
   }
 }
 

@@ -229,6 +229,25 @@ def test_attend_rows_whose_scores_are_all_minus_infinity(paged, qt, ct):
         assert (out[i].double() - want).abs().max() <= 2 * (2.2e-4 + 2 ** -16) * 4.5 + eps / 2 * 4.5
 
 
+@pytest.mark.parametrize("qt,ct", TYPES)
+def test_attend_infinite_and_nan_values_stay_in_their_element(paged, qt, ct):
+    """An infinite value under an ordinary weight makes its own output element infinite, a NaN one
+    NaN, and no other; a NaN key makes its head group's outputs NaN and no other request's."""
+    lens = [20, 20, 300]
+    k, v, table = filled(lens, 2, 16, 64, DT[ct], "hnd", 21)
+    q = (0.1 * torch.randn((3, 4, 64), generator=gen(22), device="cuda")).to(DT[qt])
+    clean = paged.attend(q, k, v, table, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    v[table[0, 0].long(), 0, 3, 9] = math.inf
+    v[table[0, 1].long(), 0, 1, 10] = -math.inf
+    v[table[0, 0].long(), 1, 5, 11] = math.nan
+    k[table[1, 0].long(), 1, 7, 0] = math.nan
+    out = paged.attend(q, k, v, table, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    assert (out[0, :2, 9] == math.inf).all() and (out[0, :2, 10] == -math.inf).all() and out[0, 2:, 11].isnan().all()
+    assert out[1, 2:].isnan().all()
+    out[0, :2, 9:11], out[0, 2:, 11], out[1, 2:] = clean[0, :2, 9:11], clean[0, 2:, 11], clean[1, 2:]
+    assert torch.equal(out, clean)
+
+
 def test_attend_strided_rows_and_neighbours_left_alone(paged):
     """Queries inside fused rows, results into a wider buffer, k and v halves of one tensor."""
     lens = [33, 0, 200]
