@@ -60,7 +60,7 @@ struct AttnK {
 
 // Workspace: per CTA a record of the partial that begins in it, then two partials per CTA
 // (the one its share begins inside of, the one it ends inside of).
-struct Joint {
+struct alignas(16) Joint {
   int i, h, pieces, pad;  // pieces: partials of (i, h), 0: none begins here
 };
 __host__ __device__ inline size_t ws_stats_off(int ctas) { return (size_t)ctas * sizeof(Joint); }
@@ -80,6 +80,13 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// 2^x; results below 2^-126 are zero.
+__device__ __forceinline__ float pow2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // What a maximum of -inf (nothing seen, or only scores of -inf) is taken as.
@@ -177,8 +184,9 @@ __device__ __forceinline__ void split_weights(float lo, float hi, uint32_t (&w)[
 // One warp's online softmax over tiles of 16-bit keys and values. Lane (g = lane / 4, t = lane % 4)
 // holds the scores of keys g and g + 8 of each 16 for heads 2t and 2t + 1 of each 8, and output
 // elements g and g + 8 of each 16 for the same heads.
-template <int HD_, typename QT_, typename CT_, int GM>
+template <int HD_, typename QT_, typename CT_, int GM_>
 struct Mma {
+  static constexpr int GM = GM_;
   using QT = QT_;
   using CT = CT_;
   static constexpr int HD = HD_;
@@ -314,7 +322,7 @@ struct Mma {
         for (int off = 4; off < 32; off <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], off));
         top[c] = fmaxf(top[c], m[nt][c]);
         const float ref = finite_or_zero(top[c]);
-        alpha[nt][c] = exp2f(m[nt][c] - ref);
+        alpha[nt][c] = pow2(m[nt][c] - ref);
         turned |= alpha[nt][c] != 1.f;
         m[nt][c] = top[c];
         top[c] = ref - kLift;
@@ -324,7 +332,7 @@ struct Mma {
       for (int mt = 0; mt < MT; mt++) {
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-          s[mt][nt][c] = exp2f(s[mt][nt][c] - top[c & 1]);
+          s[mt][nt][c] = pow2(s[mt][nt][c] - top[c & 1]);
           l[nt][c & 1] += s[mt][nt][c];
         }
         uint32_t lo[NP], hi[NP];
@@ -359,10 +367,10 @@ struct Mma {
       }
   }
 
-  // f(head, element, value of o, l) for every output of the group this lane holds, then
-  // w(head, m, l) by one lane per head; m and l over all keys the warp has seen.
-  template <class F, class W>
-  __device__ __forceinline__ void finish(int G, int lane, F&& f, W&& w) {
+  // f(head, element, o * by(l)) for every output of the group this lane holds and w(head, m, l)
+  // by one lane per head; m and l over all keys the warp has seen.
+  template <class B, class F, class W>
+  __device__ __forceinline__ void finish(int G, int lane, B&& by, F&& f, W&& w) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
@@ -373,10 +381,11 @@ struct Mma {
         for (int off = 4; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         const int head = nt * 8 + 2 * t + c;
         if (head < G) {
+          const float x = by(sum);
 #pragma unroll
           for (int j = 0; j < KS; j++) {
-            f(head, j * 16 + g, o[nt][j][c], sum);
-            f(head, j * 16 + g + 8, o[nt][j][c + 2], sum);
+            f(head, j * 16 + g, sum == 0.f ? 0.f : o[nt][j][c] * x);
+            f(head, j * 16 + g + 8, sum == 0.f ? 0.f : o[nt][j][c + 2] * x);
           }
           if (g == 0) w(head, m[nt][c], sum);
         }
@@ -418,8 +427,9 @@ __device__ __forceinline__ void sum_over(float* a, int lane) {
 // One warp's online softmax over tiles of f32 keys and values on the FMA pipes. LPK lanes share
 // a key, each E = HD / LPK of its elements (16-byte chunks LPK apart); the 32 / LPK lane groups
 // take keys in turn, each with a running maximum of its own, and are joined at the end.
-template <int HD_, int GM>
+template <int HD_, int GM_>
 struct Fma {
+  static constexpr int GM = GM_;
   using QT = float;
   using CT = float;
   static constexpr int HD = HD_;
@@ -503,13 +513,13 @@ struct Fma {
           top = fmaxf(top, s[g * KB + kk]);
         }
         const float ref = finite_or_zero(top);
-        alpha[g] = exp2f(m[g] - ref);
+        alpha[g] = pow2(m[g] - ref);
         turned |= alpha[g] != 1.f;
         m[g] = top;
         l[g] *= alpha[g];
 #pragma unroll
         for (int kk = 0; kk < KB; kk++) {
-          s[g * KB + kk] = exp2f(s[g * KB + kk] - ref);
+          s[g * KB + kk] = pow2(s[g * KB + kk] - ref);
           l[g] += s[g * KB + kk];
         }
       }
@@ -535,15 +545,15 @@ struct Fma {
     }
   }
 
-  template <class F, class W>
-  __device__ __forceinline__ void finish(int G, int lane, F&& f, W&& w) {
+  template <class B, class F, class W>
+  __device__ __forceinline__ void finish(int G, int lane, B&& by, F&& f, W&& w) {
     const int hs = lane % LPK, kg = lane / LPK;
 #pragma unroll
     for (int g = 0; g < GM; g++) {
       float top = m[g];
 #pragma unroll
       for (int off = LPK; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-      const float fac = exp2f(m[g] - finite_or_zero(top));
+      const float fac = pow2(m[g] - finite_or_zero(top));
       float sum = l[g] * fac;
 #pragma unroll
       for (int off = LPK; off < 32; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
@@ -557,8 +567,9 @@ struct Fma {
         for (int off = LPK; off < 32; off <<= 1) x[e] += __shfl_xor_sync(0xffffffffu, x[e], off);
       }
       if (g < G && g % KG == kg) {
+        const float inv = by(sum);
 #pragma unroll
-        for (int e = 0; e < E; e++) f(g, (hs + LPK * (e / 4)) * 4 + e % 4, x[e], sum);
+        for (int e = 0; e < E; e++) f(g, (hs + LPK * (e / 4)) * 4 + e % 4, sum == 0.f ? 0.f : x[e] * inv);
         if (hs == 0) w(g, top, sum);
       }
     }
@@ -567,45 +578,88 @@ struct Fma {
 
 // ---- the walk over the tiles --------------------------------------------------------------
 
-// A place in the line of tiles: tile t of kv head h of request i. Lane-parallel: every lane of
-// the warp holds the same place, and the lengths of 32 requests are kept one per lane.
+// What one (request, kv head) costs beside its tiles, in tiles: a query to load, a result to
+// write. Shares are even in tiles plus these, so that a run of very short requests is not the
+// last to finish.
+constexpr uint32_t kSegTiles = 1;
+// Requests whose lengths and running costs are kept in shared memory; more are kept in strips.
+constexpr int kLine = 512;
+
 template <int TK>
-struct Place {
-  int i, h, t, len, tiles;
-  int base, cached;  // lens[base + lane]
-
-  __device__ __forceinline__ void at_request(const AttnK& a, int cap, int req, int lane) {
-    if (req < base || req >= base + 32) {
-      base = req;
-      cached = req + lane < a.n ? min(max(ld_cg(a.lens + req + lane), 0), cap) : 0;
-    }
-    i = req;
-    len = __shfl_sync(0xffffffffu, cached, req - base);
-    tiles = (len + TK - 1) / TK;
-  }
-  __device__ __forceinline__ void next(const AttnK& a, int cap, int lane) {
-    if (++t < tiles) return;
-    t = 0;
-    if (++h < a.Hkv) return;
-    h = 0;
-    do {
-      at_request(a, cap, i + 1, lane);
-    } while (len == 0 && i + 1 < a.n);
-  }
-};
-
-struct Piece {
-  int i, h;
-  int valid, begins, ends, rest;  // rest: tiles of (i, h) behind this piece
-};
+__device__ __forceinline__ int tiles_of(int len) {
+  return len > 0 ? (len - 1) / TK + 1 : 0;
+}
 
 template <class M>
 struct Smem {
-  static constexpr int NT = M::NW * 32;
-  long long before[NT + 1];  // tiles of the requests before thread t's strip
-  long long part[33];
-  Piece piece[2 * M::NW];
-  float ml[2 * M::NW][16][2];
+  uint32_t before[kLine + 1];  // cost of the requests before each strip
+  int lens[kLine];             // up to kLine requests: their lengths
+  uint32_t part[M::NW];
+  int4 piece[2 * M::NW];  // a partial's request, kv head, flags, tiles of the two behind it
+  float2 ml[2 * M::NW][M::GM];
+};
+enum : int { kValid = 1, kBegins = 2, kEnds = 4 };
+
+// A place in the line of tiles: tile t of kv head h of request i; i == n behind the last one.
+// Every lane of a warp holds the same place.
+template <class M>
+struct Place {
+  int i, h, t, len, tiles;
+
+  __device__ __forceinline__ void at_request(const AttnK& a, const Smem<M>& sm, int cap, int req) {
+    i = req;
+    len = a.n <= kLine && !a.direct ? sm.lens[req] : min(max(ld_cg(a.lens + req), 0), cap);
+    tiles = tiles_of<M::TK>(len);
+  }
+  __device__ __forceinline__ void next(const AttnK& a, const Smem<M>& sm, int cap) {
+    if (++t < tiles) return;
+    t = 0;
+    if (!a.direct && ++h < a.Hkv) return;
+    h = 0;
+    do {
+      if (a.direct || ++i >= a.n) {
+        i = a.n;
+        return;
+      }
+      at_request(a, sm, cap, i);
+    } while (len == 0);
+  }
+  // The place at cost g of `total`; `strip` requests per entry of sm.before.
+  __device__ __forceinline__ void locate(const AttnK& a, const Smem<M>& sm, int cap, uint32_t g, uint32_t total, int strip,
+                                         int lane) {
+    h = t = 0;
+    i = a.n;
+    if (g >= total) return;
+    int st = 16 * (__popc(__ballot_sync(0xffffffffu, sm.before[16 * lane] <= g)) - 1);
+    st += __popc(__ballot_sync(0xffffffffu, lane < 16 && sm.before[st + (lane & 15)] <= g)) - 1;
+    uint32_t off = g - sm.before[st];
+    int r = st * strip;
+    if (strip > 1) {
+      for (;; r += 32) {
+        const int tl = r + lane < a.n ? tiles_of<M::TK>(min(max(ld_cg(a.lens + r + lane), 0), cap)) : 0;
+        const uint32_t own = tl ? (tl + kSegTiles) * (uint32_t)a.Hkv : 0u;
+        uint32_t run = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t u = __shfl_up_sync(0xffffffffu, run, o);
+          if (lane >= o) run += u;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, run > off);
+        if (hit) {
+          const int who = __ffs(hit) - 1;
+          off -= __shfl_sync(0xffffffffu, run - own, who);
+          r += who;
+          break;
+        }
+        off -= __shfl_sync(0xffffffffu, run, 31);
+        if (r + 32 >= a.n) return;  // not reached: sm.before holds the place
+      }
+    }
+    at_request(a, sm, cap, r);
+    const uint32_t per = (uint32_t)tiles + kSegTiles;
+    h = (int)(off / per);
+    t = max(0, (int)(off - (uint32_t)h * per) - (int)kSegTiles);
+  }
 };
 
 template <class M>
@@ -620,148 +674,149 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
   pdl_launch_dependents();
   pdl_wait();
 
-  const int cap = (int)min((long long)a.width << a.page_shift, 0x7fffffffll);
-  Place<TK> pc;
-  pc.base = -64;
-  pc.cached = 0;
-  pc.h = pc.t = 0;
-  long long todo;      // tiles of this warp
-  long long share = 0; // tiles per CTA
-  if (tid < 2 * NW) sm.piece[tid].valid = 0;
+  const int cap = a.width << a.page_shift;
+  Place<M> pc, last;   // this warp's run: [pc, last)
+  uint32_t share = 1;  // cost per CTA
+  if (tid < 2 * NW) sm.piece[tid].z = 0;
+
+  // requests without keys get their result at once
+  auto nothing = [&](long long i) {
+    QT* out = reinterpret_cast<QT*>(a.out) + i * a.out_stride;
+    for (int x = lane; x < a.H * HD; x += 32) put(out + x, 0.f);
+    if (a.lse)
+      for (int x = lane; x < a.H; x += 32) a.lse[i * a.H + x] = -INFINITY;
+  };
 
   if (a.direct) {
-    pc.at_request(a, cap, cta / a.Hkv, lane);
-    pc.h = cta % a.Hkv;
+    const int i = cta / a.Hkv;
+    if (a.status && tid == 0 && ld_cg(a.lens + i) > cap) *a.status = SX_E_RANGE;
+    pc.at_request(a, sm, cap, i);
+    if (pc.tiles == 0 && cta % a.Hkv == 0 && warp == 0) nothing(i);
     const int w0 = (int)((long long)pc.tiles * warp / NW), w1 = (int)((long long)pc.tiles * (warp + 1) / NW);
+    pc.h = last.h = cta % a.Hkv;
     pc.t = w0;
-    todo = w1 - w0;
+    last.i = i;
+    last.t = w1;
+    if (w1 == pc.tiles) last.i = a.n, last.h = last.t = 0;
+    if (w0 == w1) pc.i = last.i, pc.h = last.h, pc.t = last.t;
   } else {
-    // tiles before each strip of requests (a strip per thread) and in all
-    const int strip = (a.n + NT - 1) / NT;
-    long long mine = 0;
-    for (int i = min(a.n, tid * strip); i < min(a.n, (tid + 1) * strip); i++)
-      mine += (long long)((min(max(ld_cg(a.lens + i), 0), cap) + TK - 1) / TK) * a.Hkv;
-    long long inc = mine;
+    // cost before each strip of requests and in all
+    const int strip = (a.n + kLine - 1) / kLine;
+    constexpr int SPT = kLine / NT;  // strips per thread
+    uint32_t cost[SPT], mine = 0;
+#pragma unroll
+    for (int x = 0; x < SPT; x++) {
+      cost[x] = 0;
+      for (int y = 0; y < strip; y++) {
+        const uint32_t i = (uint32_t)(tid * SPT + x) * strip + y;
+        const int raw = i < (uint32_t)a.n ? ld_cg(a.lens + i) : 0;
+        const int len = min(max(raw, 0), cap), tl = tiles_of<TK>(len);
+        if (strip == 1) sm.lens[tid * SPT + x] = len;
+        if (tl) cost[x] += (tl + kSegTiles) * (uint32_t)a.Hkv;
+        if (raw > cap && a.status) *a.status = SX_E_RANGE;
+        // the CTAs take the empty requests in turn
+        unsigned none = __ballot_sync(0xffffffffu, i < (uint32_t)a.n && len == 0 && (int)(i % ctas) == cta);
+        while (none) {
+          const int who = __ffs(none) - 1;
+          none &= none - 1;
+          nothing(__shfl_sync(0xffffffffu, i, who));
+        }
+      }
+      mine += cost[x];
+    }
+    uint32_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+      const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += u;
     }
     if (lane == 31) sm.part[warp] = inc;
     __syncthreads();
-    long long base = 0, total = 0;
+    uint32_t base = inc - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < NW; w++) {
-      if (w < warp) base += sm.part[w];
-      total += sm.part[w];
+      const uint32_t v = sm.part[w];
+      if (w < warp) base += v;
+      total += v;
     }
-    sm.before[tid] = base + inc - mine;
-    if (tid == 0) sm.before[NT] = total;
+#pragma unroll
+    for (int x = 0; x < SPT; x++) {
+      sm.before[tid * SPT + x] = base;
+      base += cost[x];
+    }
     __syncthreads();
-    share = max((total + ctas - 1) / ctas, (long long)NW);
-    const long long c0 = min(total, share * cta), c1 = min(total, c0 + share);
-    const long long w0 = c0 + (c1 - c0) * warp / NW, w1 = c0 + (c1 - c0) * (warp + 1) / NW;
-    todo = w1 - w0;
-    if (todo > 0) {
-      // the strip, then the request, that holds tile w0
-      int st = 0;
-#pragma unroll
-      for (int x = 0; x < NT / 32; x++) {
-        const int c = x * 32 + lane;
-        const unsigned hit = __ballot_sync(0xffffffffu, sm.before[c] <= w0 && w0 < sm.before[c + 1]);
-        if (hit) st = x * 32 + __ffs(hit) - 1;
-      }
-      long long off = w0 - sm.before[st];
-      int i = st * strip;
-      for (;; i += 32) {
-        const int len = i + lane < a.n ? min(max(ld_cg(a.lens + i + lane), 0), cap) : 0;
-        long long run = (long long)((len + TK - 1) / TK) * a.Hkv;
-        const long long own = run;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long u = __shfl_up_sync(0xffffffffu, run, o);
-          if (lane >= o) run += u;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, run > off);
-        if (hit) {
-          const int who = __ffs(hit) - 1;
-          off -= __shfl_sync(0xffffffffu, run - own, who);
-          i += who;
-          break;
-        }
-        off -= __shfl_sync(0xffffffffu, run, 31);
-        if (i + 32 >= a.n) break;  // not reached: before[] holds the tile
-      }
-      pc.at_request(a, cap, i, lane);
-      pc.h = (int)(off / pc.tiles);
-      pc.t = (int)(off % pc.tiles);
-    }
+    share = max((total + ctas - 1) / ctas, (uint32_t)NW);
+    const uint32_t c0 = min((unsigned long long)total, (unsigned long long)share * cta);
+    const uint32_t c1 = min(total - c0, share);
+    // c1 warp / NW without leaving 32 bits
+    auto part = [&](int w) { return c0 + c1 / NW * w + c1 % NW * w / NW; };
+    pc.locate(a, sm, cap, part(warp), total, strip, lane);
+    last.locate(a, sm, cap, part(warp + 1), total, strip, lane);
   }
-
-  // requests without keys, and lengths that do not fit
-  for (long long i0 = cta; i0 < a.n; i0 += (long long)ctas * NT) {
-    const long long i = i0 + (long long)ctas * tid;
-    const int len = i < a.n ? ld_cg(a.lens + i) : 1;
-    if (i < a.n && len > cap && a.status) *a.status = SX_E_RANGE;
-    unsigned none = __ballot_sync(0xffffffffu, i < a.n && len <= 0);
-    while (none) {
-      const int who = __ffs(none) - 1;
-      none &= none - 1;
-      const long long j = __shfl_sync(0xffffffffu, i, who);
-      QT* out = reinterpret_cast<QT*>(a.out) + j * a.out_stride;
-      for (int x = lane; x < a.H * HD; x += 32) put(out + x, 0.f);
-      if (a.lse)
-        for (int x = lane; x < a.H; x += 32) a.lse[j * a.H + x] = -INFINITY;
-    }
-  }
-  __syncthreads();  // sm.piece is cleared
+  auto before_last = [&](const Place<M>& x) { return x.i != last.i || x.h != last.h || x.t != last.t; };
 
   uint8_t* ring = dyn + (size_t)warp * a.stages * TILE;
   const uint32_t ring_s = smem_addr(ring);
   // Where a partial at the start of a run goes. Warp 0's is the share's own first partial.
   Joint* joint = reinterpret_cast<Joint*>(a.ws);
-  float* ws_ml = reinterpret_cast<float*>(a.ws + ws_stats_off(ctas));
+  float2* ws_ml = reinterpret_cast<float2*>(a.ws + ws_stats_off(ctas));
   float* ws_o = reinterpret_cast<float*>(a.ws + ws_o_off(ctas, a.G));
   float* first_o = reinterpret_cast<float*>(dyn + (size_t)NW * a.stages * TILE);  // [NW - 1][G][HD]
 
   // the copying side runs ahead of the computing side by the ring's depth
-  Place<TK> pp = pc;
-  long long to_copy = todo;
+  Place<M> pp = pc;
   int page_of = -1, page_base = 0, pages = 0;  // request and first of the 32 pages held one per lane
   const int page_mask = (1 << a.page_shift) - 1;
   auto copy_next = [&](int stage) {
-    if (to_copy > 0) {
+    if (before_last(pp)) {
       const int key0 = pp.t * TK, p0 = key0 >> a.page_shift;
-      if (page_of != pp.i || p0 >= page_base + 32 || p0 < page_base) {
+      if (page_of != pp.i || p0 < page_base || p0 >= page_base + 32) {
         page_of = pp.i;
         page_base = p0 & ~31;
         const int idx = page_base + lane;
-        int page = -1;
+        pages = -1;
         if (idx <= (pp.len - 1) >> a.page_shift) {
-          page = ld_cg(a.table + (size_t)pp.i * a.table_stride + idx);
-          if ((unsigned)page >= (unsigned)a.n_pages) {
-            page = -1;
+          pages = ld_cg(a.table + (size_t)pp.i * a.table_stride + idx);
+          if ((unsigned)pages >= (unsigned)a.n_pages) {
+            pages = -1;
             if (a.status) *a.status = SX_E_RANGE;
           }
         }
-        pages = page;
       }
       const uint32_t dst = ring_s + stage * TILE;
-      const size_t head = (size_t)pp.h * a.head_stride;
+      const int left = pp.len - key0;
+      if (page_mask >= TK - 1) {  // the tile lies in one page
+        const int page = __shfl_sync(0xffffffffu, pages, p0 - page_base);
+        size_t off = (size_t)(page < 0 ? 0 : page) * a.page_stride + (size_t)pp.h * a.head_stride +
+                     (size_t)((key0 & page_mask) + lane / CPR) * a.token_stride + lane % CPR * 16;
+        const int rows = page < 0 ? 0 : left;
+        const size_t down = (CPR <= 32 ? 32 / CPR : 1) * a.token_stride;
 #pragma unroll
-      for (int x = 0; x < TK * CPR / 32; x++) {
-        const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR;
-        const int key = key0 + r;
-        const int page = __shfl_sync(0xffffffffu, pages, (key >> a.page_shift) - page_base);
-        const bool there = key < pp.len && page >= 0;
-        const size_t off = there ? (size_t)page * a.page_stride + head + (size_t)(key & page_mask) * a.token_stride + c * 16
-                                 : 0;
-        const uint32_t d = dst + M::at(r, c);
-        cp_async16(d, a.k + off, there ? 16 : 0);
-        cp_async16(d + TK * RB, a.v + off, there ? 16 : 0);
+        for (int x = 0; x < TK * CPR / 32; x++) {
+          const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR;
+          const int bytes = r < rows ? 16 : 0;
+          size_t at = off;
+          if constexpr (CPR > 32) at += (x & 1) * 512;
+          if (!bytes) at = 0;
+          cp_async16(dst + M::at(r, c), a.k + at, bytes);
+          cp_async16(dst + M::at(r, c) + TK * RB, a.v + at, bytes);
+          if (CPR <= 32 || (x & 1)) off += down;
+        }
+      } else {
+#pragma unroll 4
+        for (int x = 0; x < TK * CPR / 32; x++) {
+          const int idx = x * 32 + lane, r = idx / CPR, c = idx % CPR;
+          const int key = key0 + r;
+          const int page = __shfl_sync(0xffffffffu, pages, (key >> a.page_shift) - page_base);
+          const int bytes = r < left && page >= 0 ? 16 : 0;
+          const size_t at = bytes ? (size_t)page * a.page_stride + (size_t)pp.h * a.head_stride +
+                                        (size_t)(key & page_mask) * a.token_stride + c * 16
+                                  : 0;
+          cp_async16(dst + M::at(r, c), a.k + at, bytes);
+          cp_async16(dst + M::at(r, c) + TK * RB, a.v + at, bytes);
+        }
       }
-      to_copy--;
-      if (to_copy > 0) pp.next(a, cap, lane);
+      pp.next(a, sm, cap);
     }
     cp_commit();
   };
@@ -773,7 +828,7 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
 
   M mine;
   bool fresh = true, began = false;
-  for (; todo > 0; todo--) {
+  while (before_last(pc)) {
     copy_next(into);
     into = into + 1 == a.stages ? 0 : into + 1;
     if (fresh) {
@@ -783,151 +838,160 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
     }
     if (a.stages == 3)
       cp_wait<2>();
-    else if (a.stages == 2)
-      cp_wait<1>();
     else
-      cp_wait<3>();
+      cp_wait<1>();
     __syncwarp();
     const uint32_t tile = ring_s + from * TILE;
     mine.tile(tile, tile + TK * RB, min(TK, pc.len - pc.t * TK), lane);
     from = from + 1 == a.stages ? 0 : from + 1;
     __syncwarp();  // every lane has read the tile before it is overwritten
-    const bool ends = pc.t + 1 == pc.tiles;
-    if (ends || todo == 1) {
-      if (ends && began) {
-        QT* out = reinterpret_cast<QT*>(a.out) + (size_t)pc.i * a.out_stride + (size_t)pc.h * a.G * HD;
-        float* lse = a.lse ? a.lse + (size_t)pc.i * a.H + (size_t)pc.h * a.G : nullptr;
+    const int i = pc.i, h = pc.h, rest = pc.tiles - pc.t - 1;
+    pc.next(a, sm, cap);
+    const bool done = !before_last(pc);
+    if (rest == 0 || done) {
+      if (rest == 0 && began) {
+        QT* out = reinterpret_cast<QT*>(a.out) + (size_t)i * a.out_stride + (size_t)h * a.G * HD;
         mine.finish(
-            a.G, lane,
-            [&](int head, int d, float v, float sum) { put(out + head * HD + d, sum == 0.f ? 0.f : __fdiv_rn(v, sum)); },
+            a.G, lane, [&](float sum) { return sum == 0.f ? 0.f : __fdiv_rn(1.f, sum); },
+            [&](int head, int d, float v) { put(out + head * HD + d, v); },
             [&](int head, float top, float sum) {
-              if (lse) lse[head] = sum == 0.f ? -INFINITY : kLn2 * (finite_or_zero(top) + log2f(sum) - M::kLift);
+              if (a.lse)
+                a.lse[(size_t)i * a.H + (size_t)h * a.G + head] =
+                    sum == 0.f ? -INFINITY : kLn2 * (finite_or_zero(top) + log2f(sum) - M::kLift);
             });
       } else {
         // a partial: the run's last one may lie in the ring, which is then done with
-        const int slot = 2 * warp + (todo == 1);
-        const bool out_of_cta = warp == 0 && todo > 1;
-        float* dst = todo == 1    ? reinterpret_cast<float*>(ring)
+        const int slot = 2 * warp + done;
+        const bool out_of_cta = warp == 0 && !done;
+        float* dst = done         ? reinterpret_cast<float*>(ring)
                      : out_of_cta ? ws_o + (size_t)2 * cta * a.G * HD
                                   : first_o + (size_t)(warp - 1) * a.G * HD;
-        float* ml = out_of_cta ? ws_ml + (size_t)2 * cta * a.G * 2 : &sm.ml[slot][0][0];
+        float2* ml = out_of_cta ? ws_ml + (size_t)2 * cta * a.G : sm.ml[slot];
         mine.finish(
-            a.G, lane, [&](int head, int d, float v, float) { dst[head * HD + d] = v; },
-            [&](int head, float top, float sum) {
-              ml[2 * head] = top;
-              ml[2 * head + 1] = sum;
-            });
-        if (lane == 0 && !out_of_cta) {
-          Piece& p = sm.piece[slot];
-          p.i = pc.i;
-          p.h = pc.h;
-          p.begins = began;
-          p.ends = ends;
-          p.rest = pc.tiles - pc.t - 1;
-          p.valid = 1;
-        }
+            a.G, lane, [](float) { return 1.f; }, [&](int head, int d, float v) { dst[head * HD + d] = v; },
+            [&](int head, float top, float sum) { ml[head] = make_float2(top, sum); });
+        if (lane == 0 && !out_of_cta)
+          sm.piece[slot] = make_int4(i, h, kValid | (began ? kBegins : 0) | (rest == 0 ? kEnds : 0), rest);
       }
       fresh = true;
     }
-    if (todo > 1) pc.next(a, cap, lane);
   }
   cp_wait<0>();
   __syncthreads();
 
-  // join the warps' partials, in key order
-  auto piece_o = [&](int x) {
-    return (x & 1) ? reinterpret_cast<const float*>(dyn + (size_t)(x >> 1) * a.stages * TILE)
-                   : first_o + (size_t)((x >> 1) - 1) * a.G * HD;
-  };
+  // Join the warps' partials, in key order: neighbours of one (request, kv head) are a group, and
+  // the warps take the groups' query heads in turn.
+  const int4 pz = lane < 2 * NW ? sm.piece[lane] : make_int4(0, 0, 0, 0);
+  const unsigned valid = __ballot_sync(0xffffffffu, pz.z & kValid);
+  const unsigned lower = valid & ((1u << lane) - 1);
+  const int prev = lower ? 31 - __clz(lower) : 0;
+  const int prev_i = __shfl_sync(0xffffffffu, pz.x, prev), prev_h = __shfl_sync(0xffffffffu, pz.y, prev);
+  const bool same = prev_i == pz.x && prev_h == pz.y;
+  unsigned heads = __ballot_sync(0xffffffffu, (pz.z & kValid) && !(lower && same));  // first partial of each group
   bool leaves = false;
-  for (int x = 0; x < 2 * NW;) {
-    const Piece first = sm.piece[x];
-    if (!first.valid) {
-      x++;
-      continue;
+  for (int item = 0; heads; item += a.G) {
+    const int x0 = __ffs(heads) - 1;
+    heads &= heads - 1;
+    const unsigned group = valid & ~((1u << x0) - 1) & (heads ? (1u << (__ffs(heads) - 1)) - 1 : 0xffffffffu);
+    const int xn = 31 - __clz(group);
+    const int i = __shfl_sync(0xffffffffu, pz.x, x0), h = __shfl_sync(0xffffffffu, pz.y, x0);
+    const int begins = __shfl_sync(0xffffffffu, pz.z, x0) & kBegins, ends = __shfl_sync(0xffffffffu, pz.z, xn) & kEnds;
+    const int rest = __shfl_sync(0xffffffffu, pz.w, xn);
+    const int slot = 2 * cta + (begins ? 1 : 0);
+    if (begins && !ends) {
+      leaves = true;
+      if (tid == 0) *reinterpret_cast<int4*>(joint + cta) = make_int4(i, h, 1 + (int)((rest + share - 1) / share), 0);
     }
-    int last = x;
-    for (int y = x + 1; y < 2 * NW; y++) {
-      const Piece& p = sm.piece[y];
-      if (!p.valid) continue;
-      if (p.i != first.i || p.h != first.h) break;
-      last = y;
-    }
-    const Piece end = sm.piece[last];
-    const bool whole = first.begins && end.ends;
-    const int slot = 2 * cta + (first.begins ? 1 : 0);
-    for (int e = tid; e < a.G * HD; e += NT) {
-      const int head = e / HD, d = e % HD;
-      float top = -INFINITY;
-      for (int y = x; y <= last; y++)
-        if (sm.piece[y].valid) top = fmaxf(top, sm.ml[y][head][0]);
-      const float ref = finite_or_zero(top);
-      float sum = 0.f, v = 0.f;
-      for (int y = x; y <= last; y++)
-        if (sm.piece[y].valid) {
-          const float f = exp2f(sm.ml[y][head][0] - ref);
-          sum = fmaf(sm.ml[y][head][1], f, sum);
-          v = fmaf(piece_o(y)[e], f, v);
-        }
-      if (whole) {
-        put(reinterpret_cast<QT*>(a.out) + (size_t)first.i * a.out_stride + (size_t)first.h * a.G * HD + e,
-            sum == 0.f ? 0.f : __fdiv_rn(v, sum));
-        if (a.lse && d == 0)
-          a.lse[(size_t)first.i * a.H + (size_t)first.h * a.G + head] =
+    for (int head = (warp + NW - item % NW) % NW; head < a.G; head += NW) {
+      const bool in = (group >> lane) & 1;
+      const float2 ml = in ? sm.ml[lane][head] : make_float2(-INFINITY, 0.f);
+      const float top = warp_max(ml.x), ref = finite_or_zero(top);
+      const float fac = pow2(ml.x - ref), sum = warp_sum(ml.y * fac);
+      constexpr int E = HD / 32;
+      float v[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) v[e] = 0.f;
+      for (unsigned g = group; g; g &= g - 1) {
+        const int y = __ffs(g) - 1;
+        const float f = __shfl_sync(0xffffffffu, fac, y);
+        const float* o = ((y & 1) ? reinterpret_cast<const float*>(dyn + (size_t)(y >> 1) * a.stages * TILE)
+                                  : first_o + (size_t)((y >> 1) - 1) * a.G * HD) +
+                         head * HD + lane;
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = fmaf(o[32 * e], f, v[e]);
+      }
+      if (begins && ends) {
+        QT* out = reinterpret_cast<QT*>(a.out) + (size_t)i * a.out_stride + ((size_t)h * a.G + head) * HD + lane;
+        const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
+#pragma unroll
+        for (int e = 0; e < E; e++) put(out + 32 * e, sum == 0.f ? 0.f : v[e] * inv);
+        if (a.lse && lane == 0)
+          a.lse[(size_t)i * a.H + (size_t)h * a.G + head] =
               sum == 0.f ? -INFINITY : kLn2 * (ref + log2f(sum) - M::kLift);
       } else {
-        ws_o[(size_t)slot * a.G * HD + e] = v;
-        if (d == 0) {
-          ws_ml[((size_t)slot * a.G + head) * 2] = top;
-          ws_ml[((size_t)slot * a.G + head) * 2 + 1] = sum;
-        }
+        float* o = ws_o + ((size_t)slot * a.G + head) * HD + lane;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[32 * e] = v[e];
+        if (lane == 0) ws_ml[(size_t)slot * a.G + head] = make_float2(top, sum);
       }
     }
-    if (!whole && first.begins) {
-      leaves = true;
-      if (tid == 0) {
-        Joint j;
-        j.i = first.i;
-        j.h = first.h;
-        j.pieces = 1 + (int)((end.rest + share - 1) / share);
-        j.pad = 0;
-        joint[cta] = j;
-      }
-    }
-    x = last + 1;
   }
-  if (!a.direct && !leaves && tid == 0) joint[cta] = Joint{0, 0, 0, 0};
+  if (!a.direct && !leaves && tid == 0) *reinterpret_cast<int4*>(joint + cta) = make_int4(0, 0, 0, 0);
 }
 
 // Joins the partials of one query head of the (request, kv head) that begins in CTA blockIdx.x's
-// share and goes on behind it: the CTA's second partial, then the first ones of the CTAs after it.
+// share and goes on behind it: the CTA's second partial, then the first ones of the CTAs after
+// it. Groups of HD / 4 threads take the partials in turn and are added up in order.
+constexpr int kJoinThreads = 128;
 template <int HD, typename QT>
-__global__ void __launch_bounds__(HD < 128 ? 128 : HD) k_paged_join(const AttnK a, int ctas, float lift) {
+__global__ void __launch_bounds__(kJoinThreads) k_paged_join(const AttnK a, int ctas, float lift) {
+  constexpr int C = HD / 4, GROUPS = kJoinThreads / C;
+  __shared__ float4 acc[kJoinThreads];
+  __shared__ float sums[GROUPS], tops[kJoinThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
-  const int cta = blockIdx.x, head = blockIdx.y;
-  const int4 raw = __ldcg(reinterpret_cast<const int4*>(a.ws) + cta);
-  const int pieces = raw.z;
+  const int cta = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
+  const int4 joint = __ldcg(reinterpret_cast<const int4*>(a.ws) + cta);
+  const int pieces = joint.z;
   if (pieces == 0) return;
-  const float* ml = reinterpret_cast<const float*>(a.ws + ws_stats_off(ctas));
-  const float* o = reinterpret_cast<const float*>(a.ws + ws_o_off(ctas, a.G));
-  auto slot = [&](int y) { return (size_t)(y == 0 ? 2 * cta + 1 : 2 * (cta + y)) * a.G + head; };
-  const int d = threadIdx.x;
-  if (d >= HD) return;
+  const float2* ml = reinterpret_cast<const float2*>(a.ws + ws_stats_off(ctas)) + head;
+  const float4* o = reinterpret_cast<const float4*>(a.ws + ws_o_off(ctas, a.G)) + (size_t)head * C;
+  auto slot = [&](int y) { return (size_t)(y == 0 ? 2 * cta + 1 : 2 * (cta + y)) * a.G; };
   float top = -INFINITY;
-  for (int y = 0; y < pieces; y++) top = fmaxf(top, __ldcg(ml + slot(y) * 2));
+  for (int y = tid; y < pieces; y += kJoinThreads) top = fmaxf(top, __ldcg(ml + slot(y)).x);
+  top = warp_max(top);
+  if ((tid & 31) == 0) tops[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; w++) top = fmaxf(top, tops[w]);
   const float ref = finite_or_zero(top);
-  float sum = 0.f, v = 0.f;
-#pragma unroll 8
-  for (int y = 0; y < pieces; y++) {
-    const float2 s = __ldcg(reinterpret_cast<const float2*>(ml + slot(y) * 2));
-    const float f = exp2f(s.x - ref);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  const int c = tid % C, group = tid / C;
+#pragma unroll 4
+  for (int y = group; y < pieces; y += GROUPS) {
+    const float2 s = __ldcg(ml + slot(y));
+    const float4 x = __ldcg(o + slot(y) * C + c);
+    const float f = pow2(s.x - ref);
     sum = fmaf(s.y, f, sum);
-    v = fmaf(__ldcg(o + slot(y) * HD + d), f, v);
+    v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
   }
-  const size_t row = (size_t)raw.y * a.G + head;
-  put(reinterpret_cast<QT*>(a.out) + (size_t)raw.x * a.out_stride + row * HD + d, sum == 0.f ? 0.f : __fdiv_rn(v, sum));
-  if (a.lse && d == 0) a.lse[(size_t)raw.x * a.H + row] = sum == 0.f ? -INFINITY : kLn2 * (ref + log2f(sum) - lift);
+  acc[tid] = v;
+  if (c == 0) sums[group] = sum;
+  __syncthreads();
+  const size_t row = (size_t)joint.y * a.G + head;
+  float total = 0.f;
+#pragma unroll
+  for (int g = 0; g < GROUPS; g++) total += sums[g];
+  for (int d = tid; d < HD; d += kJoinThreads) {
+    float x = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; g++) x += reinterpret_cast<const float*>(acc)[g * HD + d];
+    put(reinterpret_cast<QT*>(a.out) + (size_t)joint.x * a.out_stride + row * HD + d,
+        total == 0.f ? 0.f : __fdiv_rn(x, total));
+  }
+  if (a.lse && tid == 0)
+    a.lse[(size_t)joint.x * a.H + row] = total == 0.f ? -INFINITY : kLn2 * (ref + log2f(total) - lift);
 }
 
 // Lengths up to this many keys are not split over CTAs.
@@ -947,7 +1011,7 @@ cudaError_t launch_m(AttnK a, long long bound, int sms, cudaStream_t st) {
   cudaLaunchConfig_t cfg = launch_cfg(dim3(grid), dim3(M::NW * 32), smem, st, attr);
   e = cudaLaunchKernelEx(&cfg, k_paged_attention<M>, a);
   if (e != cudaSuccess || a.direct) return e;
-  cfg = launch_cfg(dim3(sms, a.G), dim3(M::HD < 128 ? 128 : M::HD), 0, st, attr);
+  cfg = launch_cfg(dim3(sms, a.G), dim3(kJoinThreads), 0, st, attr);
   return cudaLaunchKernelEx(&cfg, k_paged_join<M::HD, typename M::QT>, a, sms, M::kLift);
 }
 

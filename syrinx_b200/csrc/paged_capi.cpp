@@ -112,6 +112,8 @@ int paged_check(const sx_paged_attention_args& a, int sms) {
     return refuse(SX_E_RANGE, "sx_paged_attention: a row's positions must be below 2^31");
   if ((int64_t)a.n_req * c.n_kv_heads > INT32_MAX)
     return refuse(SX_E_RANGE, "sx_paged_attention: n_req * n_kv_heads must be below 2^31");
+  if (paged_attention_cost(a) > UINT32_MAX)
+    return refuse(SX_E_RANGE, "sx_paged_attention: requests x kv heads x a row's positions is too large for one call");
   const int64_t width = (int64_t)a.n_heads * c.head_dim;
   if ((rc = check_row(a.q, a.q_stride, width, a.q_dtype, "sx_paged_attention: q"))) return rc;
   if ((rc = check_row(a.out, a.out_stride, width, a.q_dtype, "sx_paged_attention: out"))) return rc;
@@ -121,6 +123,14 @@ int paged_check(const sx_paged_attention_args& a, int sms) {
     return refuse(SX_E_RANGE, "sx_paged_attention: workspace holds " + std::to_string(a.workspace_bytes) + " bytes, " +
                                   std::to_string(need) + " needed");
   return SX_OK;
+}
+
+int64_t paged_attention_cost(const sx_paged_attention_args& a) {
+  const int hd = a.cache.head_dim;
+  const int keys = a.cache.dtype == SX_DTYPE_F32 ? 1024 / hd : hd == 32 ? 64 : hd == 64 ? 32 : 16;
+  const int64_t tiles = ((int64_t)a.table_width * a.cache.page_size + keys - 1) / keys + 1;
+  const int64_t rows = (int64_t)a.n_req * a.cache.n_kv_heads;
+  return rows > INT64_MAX / tiles ? INT64_MAX : rows * tiles;
 }
 
 int paged_sms(int device) {
