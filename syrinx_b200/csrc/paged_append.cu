@@ -8,6 +8,8 @@
 // interleaved pair sits in one lane and a half-head pair in lanes half a group apart.
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "paged.hpp"
 #include "sx_device.cuh"
 #include "sx_internal.hpp"
@@ -79,7 +81,7 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[E]) {
   }
 }
 
-template <int HD, typename XT, typename CT, bool IL>
+template <int HD, typename XT, typename CT, bool IL, bool NORM, int U>
 __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendK a) {
   constexpr int E = (sizeof(XT) == 4 && HD <= 128) ? 4 : 8;
   constexpr int LH = HD / E;     // lanes per head
@@ -91,9 +93,26 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendK a
   const int wpr = gridDim.y;  // warps that share a row
   const int row = blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
   if (row >= a.rows) return;
+  const uint8_t* xr = a.x + (size_t)row * a.x_stride;
+  const int h_first = blockIdx.y * HW + sub, h_step = wpr * HW;
+  float v[U][E];
+  // the loads of U heads go out together, the first ones before the row's slot is known
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int h = h0 + u * h_step;
+      if (h < n_heads && (h >= a.H || a.q)) {
+        load_vec<XT, E>(xr + ((size_t)h * HD + e0) * sizeof(XT), v[u]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; i++) v[u][i] = 0.f;
+      }
+    }
+  };
   const int slot = ld_cg(a.slots + row);
-  if (slot == -1) return;
   const int pos = a.cosv ? ld_cg(a.pos + row) : 0;
+  load(h_first);
+  if (slot == -1) return;
   if ((unsigned)slot >= (unsigned)a.n_slots || (a.cosv && (unsigned)pos >= (unsigned)a.n_pos)) {
     if (a.status && lane == 0) *a.status = SX_E_RANGE;
     return;
@@ -114,55 +133,56 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendK a
   }
   const size_t cache = (size_t)(slot >> a.page_shift) * a.page_stride +
                        (size_t)(slot & ((1 << a.page_shift) - 1)) * a.token_stride + e0;
-  const uint8_t* xr = a.x + (size_t)row * a.x_stride;
-  for (int h0 = blockIdx.y * HW; h0 < n_heads; h0 += wpr * HW) {
-    const int h = h0 + sub;
-    const bool on = h < n_heads && (h >= a.H || a.q);
-    float v[E];
+  for (int h0 = h_first; h0 - sub < n_heads; h0 += U * h_step) {
+    if (h0 != h_first) load(h0);
 #pragma unroll
-    for (int i = 0; i < E; i++) v[i] = 0.f;
-    if (on) load_vec<XT, E>(xr + ((size_t)h * HD + e0) * sizeof(XT), v);
-    const float* gain = h < a.H ? a.qn : h < a.H + a.Hkv ? a.kn : nullptr;
-    if (a.qn || a.kn) {
-      float ss = 0.f;
+    for (int u = 0; u < U; u++) {
+      const int h = h0 + u * h_step;
+      const bool on = h < n_heads && (h >= a.H || a.q);
+      if (NORM) {
+        float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < E; i++) ss = fmaf(v[i], v[i], ss);
+        for (int i = 0; i < E; i++) ss = fmaf(v[u][i], v[u][i], ss);
 #pragma unroll
-      for (int o = LH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (gain) {
-        const float den = sqrtf(__fadd_rn(__fdiv_rn(ss, (float)HD), a.eps));
+        for (int o = LH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float* gain = h < a.H ? a.qn : h < a.H + a.Hkv ? a.kn : nullptr;
+        if (gain) {
+          const float inv = __fdiv_rn(1.f, sqrtf(fmaf(ss, 1.f / HD, a.eps)));
 #pragma unroll
-        for (int i = 0; i < E; i++) v[i] = __fdiv_rn(v[i], den) * gain[e0 + i];
-      }
-    }
-    if (a.cosv) {
-      if constexpr (IL) {
-        if (h < a.H + a.Hkv) {
-#pragma unroll
-          for (int i = 0; i < E / 2; i++) {
-            const float x0 = v[2 * i], x1 = v[2 * i + 1];
-            v[2 * i] = __fsub_rn(__fmul_rn(x0, c[i]), __fmul_rn(x1, s[i]));
-            v[2 * i + 1] = __fadd_rn(__fmul_rn(x1, c[i]), __fmul_rn(x0, s[i]));
+          for (int i = 0; i < E; i += 4) {
+            const float4 g = *reinterpret_cast<const float4*>(gain + e0 + i);
+            v[u][i] *= inv * g.x, v[u][i + 1] *= inv * g.y, v[u][i + 2] *= inv * g.z, v[u][i + 3] *= inv * g.w;
           }
         }
-      } else {
-        const bool low = e0 < HD / 2;
+      }
+      if (a.cosv) {
+        if constexpr (IL) {
+          if (h < a.H + a.Hkv) {
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-          const float other = __shfl_xor_sync(0xffffffffu, v[i], LH / 2);
-          const float turned = low ? __fsub_rn(__fmul_rn(v[i], c[i]), __fmul_rn(other, s[i]))
-                                   : __fadd_rn(__fmul_rn(v[i], c[i]), __fmul_rn(other, s[i]));
-          if (h < a.H + a.Hkv) v[i] = turned;
+            for (int i = 0; i < E / 2; i++) {
+              const float x0 = v[u][2 * i], x1 = v[u][2 * i + 1];
+              v[u][2 * i] = x0 * c[i] - x1 * s[i];
+              v[u][2 * i + 1] = x1 * c[i] + x0 * s[i];
+            }
+          }
+        } else {
+          const bool low = e0 < HD / 2;
+#pragma unroll
+          for (int i = 0; i < E; i++) {
+            const float other = __shfl_xor_sync(0xffffffffu, v[u][i], LH / 2);
+            const float turned = v[u][i] * c[i] + (low ? -other : other) * s[i];
+            if (h < a.H + a.Hkv) v[u][i] = turned;
+          }
         }
       }
-    }
-    if (!on) continue;
-    if (h < a.H) {
-      store_vec<XT, E>(reinterpret_cast<XT*>(a.q + (size_t)row * a.q_stride) + (size_t)h * HD + e0, v);
-    } else {
-      const bool key = h < a.H + a.Hkv;
-      CT* base = reinterpret_cast<CT*>(key ? a.k : a.v);
-      store_vec<CT, E>(base + cache + (size_t)(h - a.H - (key ? 0 : a.Hkv)) * a.head_stride, v);
+      if (!on) continue;
+      if (h < a.H) {
+        store_vec<XT, E>(reinterpret_cast<XT*>(a.q + (size_t)row * a.q_stride) + (size_t)h * HD + e0, v[u]);
+      } else {
+        const bool key = h < a.H + a.Hkv;
+        CT* base = reinterpret_cast<CT*>(key ? a.k : a.v);
+        store_vec<CT, E>(base + cache + (size_t)(h - a.H - (key ? 0 : a.Hkv)) * a.head_stride, v[u]);
+      }
     }
   }
 }
@@ -181,8 +201,17 @@ cudaError_t launch_t(const AppendK& a, bool il, int sms, cudaStream_t st) {
   gy = gy < steps ? gy : steps;
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg = launch_cfg(dim3(gx, gy), dim3(kAppendThreads), 0, st, attr);
-  return il ? cudaLaunchKernelEx(&cfg, k_paged_append<HD, XT, CT, true>, a)
-            : cudaLaunchKernelEx(&cfg, k_paged_append<HD, XT, CT, false>, a);
+  const bool norm = a.qn || a.kn;
+  auto go = [&](auto u) {
+    constexpr int U = decltype(u)::value;
+    if (il)
+      return norm ? cudaLaunchKernelEx(&cfg, k_paged_append<HD, XT, CT, true, true, U>, a)
+                  : cudaLaunchKernelEx(&cfg, k_paged_append<HD, XT, CT, true, false, U>, a);
+    return norm ? cudaLaunchKernelEx(&cfg, k_paged_append<HD, XT, CT, false, true, U>, a)
+                : cudaLaunchKernelEx(&cfg, k_paged_append<HD, XT, CT, false, false, U>, a);
+  };
+  // a warp with one step has nothing to load ahead
+  return gy == steps ? go(std::integral_constant<int, 1>()) : go(std::integral_constant<int, 4>());
 }
 
 template <typename XT, typename CT>

@@ -28,6 +28,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "paged.hpp"
@@ -72,6 +73,17 @@ __host__ __device__ inline size_t ws_bytes(int ctas, int G, int hd) {
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Four neighbours; their 16-byte (f32) or 8-byte place is aligned.
+__device__ __forceinline__ void put4(float* p, float x, float y, float z, float w) {
+  *reinterpret_cast<float4*>(p) = make_float4(x, y, z, w);
+}
+template <typename T>
+__device__ __forceinline__ void put4(T* p, float x, float y, float z, float w) {
+  T v[4];
+  put(v, x), put(v + 1, y), put(v + 2, z), put(v + 3, w);
+  *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -677,6 +689,7 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
   const int cap = a.width << a.page_shift;
   Place<M> pc, last;   // this warp's run: [pc, last)
   uint32_t share = 1;  // cost per CTA
+  bool some_empty = false;
   if (tid < 2 * NW) sm.piece[tid].z = 0;
 
   // requests without keys get their result at once
@@ -704,6 +717,7 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
     const int strip = (a.n + kLine - 1) / kLine;
     constexpr int SPT = kLine / NT;  // strips per thread
     uint32_t cost[SPT], mine = 0;
+    bool none = false;
 #pragma unroll
     for (int x = 0; x < SPT; x++) {
       cost[x] = 0;
@@ -713,14 +727,8 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
         const int len = min(max(raw, 0), cap), tl = tiles_of<TK>(len);
         if (strip == 1) sm.lens[tid * SPT + x] = len;
         if (tl) cost[x] += (tl + kSegTiles) * (uint32_t)a.Hkv;
+        none |= i < (uint32_t)a.n && len == 0;
         if (raw > cap && a.status) *a.status = SX_E_RANGE;
-        // the CTAs take the empty requests in turn
-        unsigned none = __ballot_sync(0xffffffffu, i < (uint32_t)a.n && len == 0 && (int)(i % ctas) == cta);
-        while (none) {
-          const int who = __ffs(none) - 1;
-          none &= none - 1;
-          nothing(__shfl_sync(0xffffffffu, i, who));
-        }
       }
       mine += cost[x];
     }
@@ -731,7 +739,7 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
       if (lane >= o) inc += u;
     }
     if (lane == 31) sm.part[warp] = inc;
-    __syncthreads();
+    some_empty = __syncthreads_or(none);
     uint32_t base = inc - mine, total = 0;
 #pragma unroll
     for (int w = 0; w < NW; w++) {
@@ -826,6 +834,11 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
     into = into + 1 == a.stages ? 0 : into + 1;
   }
 
+  if (some_empty) {  // the warps of all CTAs take the requests in turn
+    for (int i = cta * NW + warp; i < a.n; i += ctas * NW)
+      if (ld_cg(a.lens + i) <= 0) nothing(i);
+  }
+
   M mine;
   bool fresh = true, began = false;
   while (before_last(pc)) {
@@ -879,60 +892,57 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
   cp_wait<0>();
   __syncthreads();
 
-  // Join the warps' partials, in key order: neighbours of one (request, kv head) are a group, and
-  // the warps take the groups' query heads in turn.
+  // Join the warps' partials, in key order: neighbours of one (request, kv head) are a group.
+  // Teams of G HD / 4 threads take the groups in turn, each thread four output elements.
   const int4 pz = lane < 2 * NW ? sm.piece[lane] : make_int4(0, 0, 0, 0);
   const unsigned valid = __ballot_sync(0xffffffffu, pz.z & kValid);
   const unsigned lower = valid & ((1u << lane) - 1);
   const int prev = lower ? 31 - __clz(lower) : 0;
   const int prev_i = __shfl_sync(0xffffffffu, pz.x, prev), prev_h = __shfl_sync(0xffffffffu, pz.y, prev);
   const bool same = prev_i == pz.x && prev_h == pz.y;
-  unsigned heads = __ballot_sync(0xffffffffu, (pz.z & kValid) && !(lower && same));  // first partial of each group
+  unsigned firsts = __ballot_sync(0xffffffffu, (pz.z & kValid) && !(lower && same));  // first partial of each group
+  const int team_size = min(NT, a.G * (HD / 4)), teams = NT / team_size, team = tid / team_size;
   bool leaves = false;
-  for (int item = 0; heads; item += a.G) {
-    const int x0 = __ffs(heads) - 1;
-    heads &= heads - 1;
-    const unsigned group = valid & ~((1u << x0) - 1) & (heads ? (1u << (__ffs(heads) - 1)) - 1 : 0xffffffffu);
-    const int xn = 31 - __clz(group);
-    const int i = __shfl_sync(0xffffffffu, pz.x, x0), h = __shfl_sync(0xffffffffu, pz.y, x0);
-    const int begins = __shfl_sync(0xffffffffu, pz.z, x0) & kBegins, ends = __shfl_sync(0xffffffffu, pz.z, xn) & kEnds;
-    const int rest = __shfl_sync(0xffffffffu, pz.w, xn);
-    const int slot = 2 * cta + (begins ? 1 : 0);
+  for (int k = 0; firsts; k++) {
+    const int x0 = __ffs(firsts) - 1;
+    firsts &= firsts - 1;
+    const unsigned group = valid & ~((1u << x0) - 1) & (firsts ? (1u << (__ffs(firsts) - 1)) - 1 : 0xffffffffu);
+    const int4 head_piece = sm.piece[x0], tail_piece = sm.piece[31 - __clz(group)];
+    const bool begins = head_piece.z & kBegins, ends = tail_piece.z & kEnds;
+    const int i = head_piece.x, h = head_piece.y, slot = 2 * cta + begins;
     if (begins && !ends) {
       leaves = true;
-      if (tid == 0) *reinterpret_cast<int4*>(joint + cta) = make_int4(i, h, 1 + (int)((rest + share - 1) / share), 0);
+      if (tid == 0)
+        *reinterpret_cast<int4*>(joint + cta) = make_int4(i, h, 1 + (int)((tail_piece.w + share - 1) / share), 0);
     }
-    for (int head = (warp + NW - item % NW) % NW; head < a.G; head += NW) {
-      const bool in = (group >> lane) & 1;
-      const float2 ml = in ? sm.ml[lane][head] : make_float2(-INFINITY, 0.f);
-      const float top = warp_max(ml.x), ref = finite_or_zero(top);
-      const float fac = pow2(ml.x - ref), sum = warp_sum(ml.y * fac);
-      constexpr int E = HD / 32;
-      float v[E];
-#pragma unroll
-      for (int e = 0; e < E; e++) v[e] = 0.f;
+    if (team != k % teams) continue;
+    for (int e = tid - team * team_size; e < a.G * (HD / 4); e += team_size) {
+      const int head = e / (HD / 4);
+      float top = -INFINITY;
+      for (unsigned g = group; g; g &= g - 1) top = fmaxf(top, sm.ml[__ffs(g) - 1][head].x);
+      const float ref = finite_or_zero(top);
+      float sum = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (unsigned g = group; g; g &= g - 1) {
         const int y = __ffs(g) - 1;
-        const float f = __shfl_sync(0xffffffffu, fac, y);
-        const float* o = ((y & 1) ? reinterpret_cast<const float*>(dyn + (size_t)(y >> 1) * a.stages * TILE)
-                                  : first_o + (size_t)((y >> 1) - 1) * a.G * HD) +
-                         head * HD + lane;
-#pragma unroll
-        for (int e = 0; e < E; e++) v[e] = fmaf(o[32 * e], f, v[e]);
+        const float2 ml = sm.ml[y][head];
+        const float4 x = reinterpret_cast<const float4*>((y & 1) ? reinterpret_cast<const float*>(dyn + (size_t)(y >> 1) * a.stages * TILE)
+                                                                 : first_o + (size_t)((y >> 1) - 1) * a.G * HD)[e];
+        const float f = pow2(ml.x - ref);
+        sum = fmaf(ml.y, f, sum);
+        v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
       }
       if (begins && ends) {
-        QT* out = reinterpret_cast<QT*>(a.out) + (size_t)i * a.out_stride + ((size_t)h * a.G + head) * HD + lane;
         const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
-#pragma unroll
-        for (int e = 0; e < E; e++) put(out + 32 * e, sum == 0.f ? 0.f : v[e] * inv);
-        if (a.lse && lane == 0)
+        if (sum == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+        put4(reinterpret_cast<QT*>(a.out) + (size_t)i * a.out_stride + (size_t)h * a.G * HD + 4 * e, v.x * inv, v.y * inv,
+             v.z * inv, v.w * inv);
+        if (a.lse && e % (HD / 4) == 0)
           a.lse[(size_t)i * a.H + (size_t)h * a.G + head] =
               sum == 0.f ? -INFINITY : kLn2 * (ref + log2f(sum) - M::kLift);
       } else {
-        float* o = ws_o + ((size_t)slot * a.G + head) * HD + lane;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[32 * e] = v[e];
-        if (lane == 0) ws_ml[(size_t)slot * a.G + head] = make_float2(top, sum);
+        reinterpret_cast<float4*>(ws_o)[(size_t)slot * a.G * (HD / 4) + e] = v;
+        if (e % (HD / 4) == 0) ws_ml[(size_t)slot * a.G + head] = make_float2(top, sum);
       }
     }
   }
@@ -1004,8 +1014,20 @@ cudaError_t launch_m(AttnK a, long long bound, int sms, cudaStream_t st) {
   a.stages = std::min(3, (kMaxSmem - (int)sizeof(Smem<M>) - 128 - partials) / (M::NW * TILE));
   a.direct = bound <= kDirectLen;
   const size_t smem = (size_t)M::NW * a.stages * TILE + partials;
-  cudaError_t e = cudaFuncSetAttribute(k_paged_attention<M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // the joining kernel asks for the same split of L1 and shared memory, so that it can be resident
+  // (and wait) while the first one runs
+  static std::atomic<uint64_t> ready{0};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
+  if (device >= 64 || !(ready.load(std::memory_order_acquire) >> device & 1)) {
+    constexpr int most = kMaxSmem - (int)sizeof(Smem<M>) - 128;
+    if ((e = cudaFuncSetAttribute(k_paged_attention<M>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute(k_paged_join<M::HD, typename M::QT>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                  cudaSharedmemCarveoutMaxShared)) != cudaSuccess)
+      return e;
+    if (device < 64) ready.fetch_or(1ull << device, std::memory_order_release);
+  }
   const int grid = a.direct ? a.n * a.Hkv : sms;
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t cfg = launch_cfg(dim3(grid), dim3(M::NW * 32), smem, st, attr);
