@@ -8,8 +8,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 
-from .configs import (SxCodecInfo, SxModelDesc, SxPagedAppendArgs, SxPagedAttentionArgs, SxPagedPlanArgs,
-                      SxSamplingParams)
+from .configs import SxCodecInfo, SxModelDesc, SxSamplingParams
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libsyrinx_b200.so")
 
@@ -69,10 +68,10 @@ SIGNATURES = {
     "sx_codec_set_stream": (C.c_int, [C.c_void_p, C.c_void_p]),
     "sx_codec_decode": (C.c_int, [C.c_void_p, _u32p, C.c_int32, C.c_int32, _f32p, C.c_size_t]),
     "sx_codec_decode_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p]),
-    # include/syrinx_paged.h
-    "sx_paged_plan": (C.c_int, [C.POINTER(SxPagedPlanArgs), C.c_int32, C.c_void_p]),
-    "sx_paged_append": (C.c_int, [C.POINTER(SxPagedAppendArgs), C.c_int32, C.c_void_p]),
-    "sx_paged_attention": (C.c_int, [C.POINTER(SxPagedAttentionArgs), C.c_int32, C.c_void_p]),
+    # include/syrinx_paged.h (the argument structs by address: ctypes structures or packed bytes)
+    "sx_paged_plan": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p]),
+    "sx_paged_append": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p]),
+    "sx_paged_attention": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p]),
     "sx_paged_attention_workspace": (C.c_int, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_size_t)]),
 }
 

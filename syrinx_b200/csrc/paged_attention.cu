@@ -32,6 +32,7 @@
 #include <type_traits>
 
 #include "paged.hpp"
+#include "paged_device.cuh"
 #include "sx_device.cuh"
 #include "sx_internal.hpp"
 
@@ -83,15 +84,6 @@ __device__ __forceinline__ void put4(T* p, float x, float y, float z, float w) {
   T v[4];
   put(v, x), put(v + 1, y), put(v + 2, z), put(v + 3, w);
   *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
-}
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // 2^x; results below 2^-126 are zero.

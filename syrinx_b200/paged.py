@@ -16,12 +16,12 @@ the `status` tensors (include/syrinx_paged.h).
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
 from . import _lib
-from .configs import (SX_DTYPE_BF16, SX_DTYPE_F32, SxPagedAppendArgs, SxPagedAttentionArgs, SxPagedCache,
-                      SxPagedPlanArgs)
+from .configs import SX_DTYPE_BF16, SX_DTYPE_F32, SxPagedAppendArgs, SxPagedAttentionArgs, SxPagedPlanArgs
 
 SX_DTYPE_F16 = 1
 _DTYPES = {torch.float32: SX_DTYPE_F32, torch.float16: SX_DTYPE_F16, torch.bfloat16: SX_DTYPE_BF16}
@@ -33,22 +33,38 @@ def _need(ok: bool, msg: str) -> None:
         raise ValueError(msg)
 
 
-def _device(t: torch.Tensor, *others) -> int:
-    dev = t.device
-    _need(dev.type == "cuda", "the tensors must be on a CUDA device")
-    for o in others:
-        _need(o is None or o.device == dev, "the tensors must be on one device")
-    return dev.index
+# cudaStream_t of torch's current stream on a device; the public call builds a Stream object for it,
+# a quarter of a small operator's host time
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_I32, _F32 = torch.int32, torch.float32
 
 
-def _stream(index: int) -> int:
-    return torch.cuda.current_stream(index).cuda_stream
+# The argument structs of include/syrinx_paged.h, packed in one go (native sizes and alignment; the
+# ctypes structures of configs.py spell the same fields out).
+_CACHE = "PPqqqiiiiii"
+_PLAN_ARGS = struct.Struct("@12Pq6i0q")
+_APPEND_ARGS = struct.Struct("@" + _CACHE + "9P2qf5i0q")
+_ATTEND_ARGS = struct.Struct("@" + _CACHE + "7PN3q5if0q")
+for _s, _c in ((_PLAN_ARGS, SxPagedPlanArgs), (_APPEND_ARGS, SxPagedAppendArgs), (_ATTEND_ARGS, SxPagedAttentionArgs)):
+    assert _s.size == C.sizeof(_c), "argument struct out of step with include/syrinx_paged.h"
+
+
+def _device(*tensors) -> int:
+    """The one CUDA device that the tensors (None: left out) are on."""
+    dev = tensors[0].get_device()
+    if dev < 0:
+        raise ValueError("the tensors must be on a CUDA device")
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError("the tensors must be on one device")
+    return dev
 
 
 def _ints(t: torch.Tensor, name: str, least: int) -> int:
-    _need(t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= least,
-          f"{name}: a contiguous int32 tensor of at least {least} entries")
-    return t.data_ptr()
+    if t.dtype is _I32 and t.is_contiguous() and t.numel() >= least:
+        return t.data_ptr()
+    raise ValueError(f"{name}: a contiguous int32 tensor of at least {least} entries")
 
 
 def _row(t: torch.Tensor) -> int:
@@ -57,27 +73,24 @@ def _row(t: torch.Tensor) -> int:
 
 
 def _table(t: torch.Tensor, n: int) -> int:
-    _need(t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] >= n and t.shape[1] >= 1 and t.stride(1) == 1,
-          "table: int32 [requests, pages] with contiguous rows")
+    s = t.shape
+    if t.dtype is not _I32 or len(s) != 2 or s[0] < n or s[1] < 1 or t.stride(1) != 1:
+        raise ValueError("table: int32 [requests, pages] with contiguous rows")
     return t.data_ptr()
 
 
-def _cache(c: SxPagedCache, k: torch.Tensor, v: torch.Tensor, layout: str) -> None:
-    """k and v pages: [pages, kv heads, page, head_dim] ("hnd") or [pages, page, kv heads, head_dim] ("nhd")."""
-    _need(k.dim() == 4 and v.shape == k.shape and v.dtype == k.dtype and v.stride() == k.stride(),
-          "k and v: four dimensions, with the same shape, type and strides")
-    dtype = _DTYPES.get(k.dtype)
-    _need(dtype is not None, "k and v must be float32, float16 or bfloat16")
-    s, st = k.shape, k.stride()
-    _need(st[3] == 1 or s[3] == 1, "k and v: the head dimension must be contiguous")
+def _cache(k: torch.Tensor, v: torch.Tensor, layout: str) -> tuple:
+    """The fields of sx_paged_cache: k and v pages are [pages, kv heads, page, head_dim] ("hnd") or
+    [pages, page, kv heads, head_dim] ("nhd")."""
+    s, st, dtype = k.shape, k.stride(), _DTYPES.get(k.dtype)
+    if len(s) != 4 or v.shape != s or v.dtype is not k.dtype or v.stride() != st:
+        raise ValueError("k and v: four dimensions, with the same shape, type and strides")
+    if dtype is None or st[3] != 1:
+        raise ValueError("k and v: float32, float16 or bfloat16, the head dimension contiguous")
     if layout == "hnd":
-        heads, page, head_stride, token_stride = s[1], s[2], st[1], st[2]
-    else:
-        _need(layout == "nhd", 'layout must be "hnd" or "nhd"')
-        heads, page, head_stride, token_stride = s[2], s[1], st[2], st[1]
-    c.k, c.v = k.data_ptr(), v.data_ptr()
-    c.page_stride, c.head_stride, c.token_stride = st[0], head_stride, token_stride
-    c.dtype, c.n_pages, c.page_size, c.n_kv_heads, c.head_dim = dtype, s[0], page, heads, s[3]
+        return k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], dtype, s[0], s[2], s[1], s[3], 0
+    _need(layout == "nhd", 'layout must be "hnd" or "nhd"')
+    return k.data_ptr(), v.data_ptr(), st[0], st[2], st[1], dtype, s[0], s[1], s[2], s[3], 0
 
 
 def plan(lens, delta, table, free_pages, n_free, *, page_size: int, slots=None, tok_seq=None, tok_pos=None,
@@ -86,29 +99,22 @@ def plan(lens, delta, table, free_pages, n_free, *, page_size: int, slots=None, 
     `free_pages` [pages] and `n_free` [1] are int32; `lens_out` and `n_free_out` default to updating
     `lens` and `n_free` in place. Returns `status` [4]: code, new tokens, pages taken, pages free.
     `check(status)` raises if the code is not SX_OK."""
-    n = lens.shape[0]
+    n, most = lens.shape[0], 0 if slots is None else slots.shape[0]
     lens_out = lens if lens_out is None else lens_out
     n_free_out = n_free if n_free_out is None else n_free_out
-    dev = _device(lens, delta, table, free_pages, n_free, slots, tok_seq, tok_pos, starts, lens_out, n_free_out, status)
     if status is None:
         status = torch.empty(4, dtype=torch.int32, device=lens.device)
-    most = 0 if slots is None else slots.shape[0]
-    a = SxPagedPlanArgs()
-    a.lens_in, a.delta, a.n_free_in = _ints(lens, "lens", n), _ints(delta, "delta", n), _ints(n_free, "n_free", 1)
-    a.lens_out, a.n_free_out = _ints(lens_out, "lens_out", n), _ints(n_free_out, "n_free_out", 1)
-    a.table, a.free_pages = _table(table, n), _ints(free_pages, "free_pages", 1)
-    if most:
-        a.slots = _ints(slots, "slots", most)
-    if tok_seq is not None:
-        a.tok_seq = _ints(tok_seq, "tok_seq", max(1, most))
-    if tok_pos is not None:
-        a.tok_pos = _ints(tok_pos, "tok_pos", max(1, most))
-    if starts is not None:
-        a.starts = _ints(starts, "starts", n + 1)
-    a.status = _ints(status, "status", 4)
-    a.table_stride, a.table_width = _row(table), table.shape[1]
-    a.n_req, a.n_pages, a.page_size, a.max_tokens = n, free_pages.shape[0], page_size, most
-    _lib.check(_lib.lib().sx_paged_plan(C.byref(a), dev, _stream(dev)))
+    dev = _device(lens, delta, table, free_pages, n_free, slots, tok_seq, tok_pos, starts, lens_out, n_free_out, status)
+    _need(most <= 0 or slots.dim() == 1, "slots: one dimension")
+    least = max(1, most)
+    args = _PLAN_ARGS.pack(
+        _ints(lens, "lens", n), _ints(delta, "delta", n), _ints(n_free, "n_free", 1), _ints(lens_out, "lens_out", n),
+        _ints(n_free_out, "n_free_out", 1), _table(table, n), _ints(free_pages, "free_pages", 1),
+        _ints(slots, "slots", most) if most else 0, 0 if tok_seq is None else _ints(tok_seq, "tok_seq", least),
+        0 if tok_pos is None else _ints(tok_pos, "tok_pos", least),
+        0 if starts is None else _ints(starts, "starts", n + 1), _ints(status, "status", 4),
+        _row(table), table.shape[1], n, free_pages.shape[0], page_size, most, 0)
+    _lib.check(_lib.lib().sx_paged_plan(args, dev, _stream(dev)))
     return status
 
 
@@ -117,36 +123,33 @@ def append(x, k, v, slots, *, n_heads: int, positions=None, cos=None, sin=None, 
     """Norm, rotate and scatter the rows [query heads | key heads | value heads] of `x` (sx_paged_append).
     Keys and values go to `k` / `v` at `slots`; the query heads are returned, in `out` [rows, n_heads *
     head_dim] where it is given. Rows with slot -1 are left out of both."""
-    c = SxPagedAppendArgs()
-    _cache(c.cache, k, v, layout)
-    dev = _device(x, k, v, slots, positions, cos, sin, q_norm, k_norm, out, status)
-    rows, hd = x.shape[0], c.cache.head_dim
-    _need(x.dim() == 2 and x.stride(1) == 1 and x.dtype in _DTYPES, "x: floating [rows, heads * head_dim]")
-    _need(x.shape[1] == (n_heads + 2 * c.cache.n_kv_heads) * hd, "x: a row is n_heads + 2 kv heads of head_dim")
+    cache = _cache(k, v, layout)
+    rows, width = x.shape
+    hkv, hd, dtype = cache[8], cache[9], x.dtype
+    _need(dtype in _DTYPES and x.stride(1) == 1, "x: floating [rows, heads * head_dim]")
+    _need(width == (n_heads + 2 * hkv) * hd, "x: a row is n_heads + 2 kv heads of head_dim")
     if out is None:
-        out = torch.empty((rows, n_heads * hd), dtype=x.dtype, device=x.device)
-    else:
-        _need(out.dim() == 2 and out.shape[0] >= rows and out.shape[1] == n_heads * hd and out.dtype == x.dtype
-              and (out.stride(1) == 1 or out.shape[1] == 1), "out: [rows, n_heads * head_dim] of x's type")
-    c.x, c.x_stride, c.x_dtype = x.data_ptr(), _row(x), _DTYPES[x.dtype]
-    if n_heads:
-        c.q_out, c.q_stride = out.data_ptr(), _row(out)
-    c.slots = _ints(slots, "slots", rows)
-    if positions is not None:
-        c.positions = _ints(positions, "positions", rows)
+        out = torch.empty((rows, n_heads * hd), dtype=dtype, device=x.device)
+    elif out.dim() != 2 or out.shape[0] < rows or out.shape[1] != n_heads * hd or out.dtype is not dtype or (
+            out.stride(1) != 1 and out.shape[1] > 1):
+        raise ValueError("out: [rows, n_heads * head_dim] of x's type")
+    dev = _device(x, k, v, slots, positions, cos, sin, q_norm, k_norm, out, status)
+    n_pos = 0
     if cos is not None or sin is not None:
-        for t in (cos, sin):
-            _need(t is not None and t.dtype == torch.float32 and t.is_contiguous() and t.dim() == 2
-                  and t.shape == cos.shape and t.shape[1] == hd // 2, "cos and sin: float32 [positions, head_dim / 2]")
-        c.cos, c.sin, c.n_positions = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if t is not None:
-            _need(t.dtype == torch.float32 and t.is_contiguous() and t.numel() == hd, f"{name}: float32 [head_dim]")
-            setattr(c, name, t.data_ptr())
-    if status is not None:
-        c.status = _ints(status, "status", 1)
-    c.eps, c.n_rows, c.n_heads, c.interleaved = eps, rows, n_heads, int(interleaved)
-    _lib.check(_lib.lib().sx_paged_append(C.byref(c), dev, _stream(dev)))
+        _need(cos is not None and sin is not None and cos.dtype is _F32 and sin.dtype is _F32
+              and cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == hd // 2 and cos.is_contiguous()
+              and sin.is_contiguous(), "cos and sin: float32 [positions, head_dim / 2]")
+        n_pos = cos.shape[0]
+    for t in (q_norm, k_norm):
+        _need(t is None or (t.dtype is _F32 and t.numel() == hd and t.is_contiguous()),
+              "q_norm and k_norm: float32 [head_dim]")
+    args = _APPEND_ARGS.pack(
+        *cache, x.data_ptr(), out.data_ptr() if n_heads else 0, _ints(slots, "slots", rows),
+        0 if positions is None else _ints(positions, "positions", rows), cos.data_ptr() if n_pos else 0,
+        sin.data_ptr() if n_pos else 0, 0 if q_norm is None else q_norm.data_ptr(),
+        0 if k_norm is None else k_norm.data_ptr(), 0 if status is None else _ints(status, "status", 1),
+        _row(x), _row(out), eps, _DTYPES[dtype], rows, n_heads, n_pos, int(interleaved))
+    _lib.check(_lib.lib().sx_paged_append(args, dev, _stream(dev)))
     return out
 
 
@@ -166,37 +169,34 @@ def attend(q, k, v, table, lens, *, scale: float | None = None, layout: str = "h
     `lens[i]` positions of the pages in `table[i]`; returns `out`, of q's shape and type. `scale` defaults to
     1 / sqrt(head_dim), `lse` [n, heads] float32 receives log sum exp. Without `workspace` (a tensor of
     `workspace_bytes`) one is taken from torch's allocator for the call."""
-    a = SxPagedAttentionArgs()
-    _cache(a.cache, k, v, layout)
-    dev = _device(q, k, v, table, lens, out, lse, workspace, status)
-    hd = a.cache.head_dim
-    _need(q.dim() == 3 and q.shape[2] == hd and q.dtype in _DTYPES, "q: floating [requests, heads, head_dim]")
-    n, heads = q.shape[0], q.shape[1]
-    _need(q.stride(2) == 1 and (heads == 1 or q.stride(1) == hd), "q: a request's heads must be contiguous")
+    cache = _cache(k, v, layout)
+    hkv, hd, dtype, shape = cache[8], cache[9], q.dtype, q.shape
+    if len(shape) != 3 or shape[2] != hd or dtype not in _DTYPES:
+        raise ValueError("q: floating [requests, heads, head_dim]")
+    n, heads = shape[0], shape[1]
+    if q.stride(2) != 1 or (heads > 1 and q.stride(1) != hd):
+        raise ValueError("q: a request's heads must be contiguous")
     if out is None:
-        out = torch.empty((n, heads, hd), dtype=q.dtype, device=q.device)
-    else:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
-              and (heads == 1 or out.stride(1) == hd), "out: q's shape and type, a request's heads contiguous")
+        out = torch.empty((n, heads, hd), dtype=dtype, device=q.device)
+    elif out.shape != shape or out.dtype is not dtype or out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd):
+        raise ValueError("out: q's shape and type, a request's heads contiguous")
+    dev = _device(q, k, v, table, lens, out, lse, workspace, status)
     if n == 0:
         return out
-    bytes_ = workspace_bytes(heads, a.cache.n_kv_heads, hd, dev)
+    size = _WORKSPACE.get((heads, hkv, hd, dev)) or workspace_bytes(heads, hkv, hd, dev)
     if workspace is None:
-        workspace = torch.empty(bytes_, dtype=torch.uint8, device=q.device)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
     else:
         _need(workspace.is_contiguous(), "workspace must be contiguous")
-    a.q, a.out, a.q_stride, a.out_stride = q.data_ptr(), out.data_ptr(), _row(q), _row(out)
-    if lse is not None:
-        _need(lse.dtype == torch.float32 and lse.is_contiguous() and lse.numel() == n * heads,
-              "lse: float32 [requests, heads]")
-        a.lse = lse.data_ptr()
-    a.table, a.lens = _table(table, n), _ints(lens, "lens", n)
-    if status is not None:
-        a.status = _ints(status, "status", 1)
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    a.table_stride, a.table_width, a.n_req, a.n_heads = _row(table), table.shape[1], n, heads
-    a.q_dtype, a.max_len, a.scale = _DTYPES[q.dtype], max_len, hd ** -0.5 if scale is None else scale
-    _lib.check(_lib.lib().sx_paged_attention(C.byref(a), dev, _stream(dev)))
+        size = workspace.numel() * workspace.element_size()
+    if lse is not None and (lse.dtype is not _F32 or lse.numel() != n * heads or not lse.is_contiguous()):
+        raise ValueError("lse: float32 [requests, heads]")
+    args = _ATTEND_ARGS.pack(
+        *cache, q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), _table(table, n),
+        _ints(lens, "lens", n), 0 if status is None else _ints(status, "status", 1), workspace.data_ptr(), size,
+        _row(q), _row(out), _row(table), table.shape[1], n, heads, _DTYPES[dtype], max_len,
+        hd ** -0.5 if scale is None else scale)
+    _lib.check(_lib.lib().sx_paged_attention(args, dev, _stream(dev)))
     return out
 
 
