@@ -55,7 +55,6 @@ struct AttnK {
   long long page_stride, head_stride, token_stride;  // bytes
   long long table_stride;
   int n, Hkv, G, H, page_shift, width, n_pages;
-  int stages;  // tiles in a warp's ring
   int direct;  // 1: CTA c is (request c / Hkv, kv head c % Hkv); nothing is split over CTAs
   float scale;
 };
@@ -586,6 +585,10 @@ struct Fma {
 // write. Shares are even in tiles plus these, so that a run of very short requests is not the
 // last to finish.
 constexpr uint32_t kSegTiles = 1;
+// Tiles in a warp's ring: one is computed while one is copied. With 8 warps that is 64 to 128 KB in
+// flight per SM. Three took 2.6 us longer at 168 MB: the first tiles of all warps queue up, and
+// every warp waits for them.
+constexpr int kStages = 2;
 // Requests whose lengths and running costs are kept in shared memory; more are kept in strips.
 constexpr int kLine = 512;
 
@@ -679,7 +682,7 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
   pdl_wait();
 
   const int cap = a.width << a.page_shift;
-  Place<M> pc, last;   // this warp's run: [pc, last)
+  Place<M> pc, last = {};  // this warp's run: [pc, last)
   uint32_t share = 1;  // cost per CTA
   bool some_empty = false;
   if (tid < 2 * NW) sm.piece[tid].z = 0;
@@ -750,18 +753,21 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
     const uint32_t c1 = min(total - c0, share);
     // c1 warp / NW without leaving 32 bits
     auto part = [&](int w) { return c0 + c1 / NW * w + c1 % NW * w / NW; };
-    pc.locate(a, sm, cap, part(warp), total, strip, lane);
-    last.locate(a, sm, cap, part(warp + 1), total, strip, lane);
+#pragma unroll 1
+    for (int x = 0; x < 2; x++) {
+      pc = last;
+      last.locate(a, sm, cap, part(warp + x), total, strip, lane);
+    }
   }
   auto before_last = [&](const Place<M>& x) { return x.i != last.i || x.h != last.h || x.t != last.t; };
 
-  uint8_t* ring = dyn + (size_t)warp * a.stages * TILE;
+  uint8_t* ring = dyn + (size_t)warp * kStages * TILE;
   const uint32_t ring_s = smem_addr(ring);
   // Where a partial at the start of a run goes. Warp 0's is the share's own first partial.
   Joint* joint = reinterpret_cast<Joint*>(a.ws);
   float2* ws_ml = reinterpret_cast<float2*>(a.ws + ws_stats_off(ctas));
   float* ws_o = reinterpret_cast<float*>(a.ws + ws_o_off(ctas, a.G));
-  float* first_o = reinterpret_cast<float*>(dyn + (size_t)NW * a.stages * TILE);  // [NW - 1][G][HD]
+  float* first_o = reinterpret_cast<float*>(dyn + (size_t)NW * kStages * TILE);  // [NW - 1][G][HD]
 
   // the copying side runs ahead of the computing side by the ring's depth
   Place<M> pp = pc;
@@ -820,35 +826,30 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
     }
     cp_commit();
   };
-  int into = 0, from = 0;
-  for (int x = 0; x < a.stages - 1; x++) {
-    copy_next(into);
-    into = into + 1 == a.stages ? 0 : into + 1;
-  }
-
-  if (some_empty) {  // the warps of all CTAs take the requests in turn
-    for (int i = cta * NW + warp; i < a.n; i += ctas * NW)
-      if (ld_cg(a.lens + i) <= 0) nothing(i);
-  }
-
   M mine;
-  bool fresh = true, began = false;
-  while (before_last(pc)) {
-    copy_next(into);
-    into = into + 1 == a.stages ? 0 : into + 1;
+  int stage = 0;
+  bool lead = true, fresh = true, began = false;
+  for (;;) {
+    copy_next(stage);  // one tile ahead of the one computed
+    stage ^= 1;
+    if (lead) {
+      lead = false;
+      if (some_empty) {  // the warps of all CTAs take the requests in turn
+        for (int i = cta * NW + warp; i < a.n; i += ctas * NW)
+          if (ld_cg(a.lens + i) <= 0) nothing(i);
+      }
+      continue;
+    }
+    if (!before_last(pc)) break;
     if (fresh) {
       mine.start(a, pc.i, pc.h, lane);
       began = pc.t == 0;
       fresh = false;
     }
-    if (a.stages == 3)
-      cp_wait<2>();
-    else
-      cp_wait<1>();
+    cp_wait<1>();
     __syncwarp();
-    const uint32_t tile = ring_s + from * TILE;
+    const uint32_t tile = ring_s + stage * TILE;
     mine.tile(tile, tile + TK * RB, min(TK, pc.len - pc.t * TK), lane);
-    from = from + 1 == a.stages ? 0 : from + 1;
     __syncwarp();  // every lane has read the tile before it is overwritten
     const int i = pc.i, h = pc.h, rest = pc.tiles - pc.t - 1;
     pc.next(a, sm, cap);
@@ -911,14 +912,16 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
     for (int e = tid - team * team_size; e < a.G * (HD / 4); e += team_size) {
       const int head = e / (HD / 4);
       float top = -INFINITY;
+#pragma unroll 1
       for (unsigned g = group; g; g &= g - 1) top = fmaxf(top, sm.ml[__ffs(g) - 1][head].x);
       const float ref = finite_or_zero(top);
       float sum = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
       for (unsigned g = group; g; g &= g - 1) {
         const int y = __ffs(g) - 1;
         const float2 ml = sm.ml[y][head];
-        const float4 x = reinterpret_cast<const float4*>((y & 1) ? reinterpret_cast<const float*>(dyn + (size_t)(y >> 1) * a.stages * TILE)
+        const float4 x = reinterpret_cast<const float4*>((y & 1) ? reinterpret_cast<const float*>(dyn + (size_t)(y >> 1) * kStages * TILE)
                                                                  : first_o + (size_t)((y >> 1) - 1) * a.G * HD)[e];
         const float f = pow2(ml.x - ref);
         sum = fmaf(ml.y, f, sum);
@@ -1003,9 +1006,8 @@ template <class M>
 cudaError_t launch_m(AttnK a, long long bound, int sms, cudaStream_t st) {
   constexpr int TILE = 2 * M::TK * M::RB;
   const int partials = (M::NW - 1) * a.G * M::HD * 4;
-  a.stages = std::min(3, (kMaxSmem - (int)sizeof(Smem<M>) - 128 - partials) / (M::NW * TILE));
   a.direct = bound <= kDirectLen;
-  const size_t smem = (size_t)M::NW * a.stages * TILE + partials;
+  const size_t smem = (size_t)M::NW * kStages * TILE + partials;
   // the joining kernel asks for the same split of L1 and shared memory, so that it can be resident
   // (and wait) while the first one runs
   static std::atomic<uint64_t> ready{0};
@@ -1082,7 +1084,6 @@ cudaError_t launch_paged_attention(const sx_paged_attention_args& a, int sms, cu
   k.page_shift = __builtin_ctz((unsigned)a.cache.page_size);
   k.width = a.table_width;
   k.n_pages = a.cache.n_pages;
-  k.stages = 0;
   k.direct = 0;
   k.scale = a.scale;
   long long bound = (long long)a.table_width * a.cache.page_size;
