@@ -591,6 +591,8 @@ constexpr uint32_t kSegTiles = 1;
 constexpr int kStages = 2;
 // Requests whose lengths and running costs are kept in shared memory; more are kept in strips.
 constexpr int kLine = 512;
+// Up to this many requests every warp sums the costs itself.
+constexpr int kFewRequests = 128;
 
 template <int TK>
 __device__ __forceinline__ int tiles_of(int len) {
@@ -662,6 +664,13 @@ struct Place {
         if (r + 32 >= a.n) return;  // not reached: sm.before holds the place
       }
     }
+    at_cost(a, sm, cap, r, off);
+  }
+  // The place at cost `off` of request r (-1: behind the last one).
+  __device__ __forceinline__ void at_cost(const AttnK& a, const Smem<M>& sm, int cap, int r, uint32_t off) {
+    h = t = 0;
+    i = a.n;
+    if (r < 0) return;
     at_request(a, sm, cap, r);
     const uint32_t per = (uint32_t)tiles + kSegTiles;
     h = (int)(off / per);
@@ -695,6 +704,15 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
       for (int x = lane; x < a.H; x += 32) a.lse[i * a.H + x] = -INFINITY;
   };
 
+  // this warp's part [lo, hi) of the CTA's even share of the total cost
+  auto run_of = [&](uint32_t total, uint32_t& lo, uint32_t& hi) {
+    share = max((total + ctas - 1) / ctas, (uint32_t)NW);
+    const uint32_t c0 = min((unsigned long long)total, (unsigned long long)share * cta);
+    const uint32_t c = min(total - c0, share);
+    lo = c0 + c / NW * warp + c % NW * warp / NW;  // c warp / NW without leaving 32 bits
+    hi = c0 + c / NW * (warp + 1) + c % NW * (warp + 1) / NW;
+  };
+
   if (a.direct) {
     const int i = cta / a.Hkv;
     if (a.status && tid == 0 && ld_cg(a.lens + i) > cap) *a.status = SX_E_RANGE;
@@ -707,6 +725,52 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
     last.t = w1;
     if (w1 == pc.tiles) last.i = a.n, last.h = last.t = 0;
     if (w0 == w1) pc.i = last.i, pc.h = last.h, pc.t = last.t;
+  } else if (a.n <= kFewRequests) {
+    // every warp for itself, 32 requests at a time and without a barrier: the running costs in
+    // registers, the lengths in shared memory (all warps write the same)
+    constexpr int R = kFewRequests / 32;
+    uint32_t before[R], own[R], total = 0;
+#pragma unroll
+    for (int x = 0; x < R; x++) own[x] = x * 32 + lane < a.n ? (uint32_t)ld_cg(a.lens + x * 32 + lane) : 0u;
+#pragma unroll
+    for (int x = 0; x < R; x++) {
+      if (x * 32 >= a.n) break;
+      const bool in = x * 32 + lane < a.n;
+      const int len = min(max((int)own[x], 0), cap), tl = tiles_of<TK>(len);
+      if ((int)own[x] > cap && a.status) *a.status = SX_E_RANGE;
+      some_empty |= __any_sync(0xffffffffu, in && len == 0);
+      if (in) sm.lens[x * 32 + lane] = len;
+      own[x] = tl ? (tl + kSegTiles) * (uint32_t)a.Hkv : 0u;
+      uint32_t run = own[x];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += u;
+      }
+      before[x] = total + run - own[x];
+      total += __shfl_sync(0xffffffffu, run, 31);
+    }
+    __syncwarp();
+    uint32_t lo, hi;
+    run_of(total, lo, hi);
+#pragma unroll 1
+    for (int y = 0; y < 2; y++) {
+      const uint32_t g = y ? hi : lo;
+      int r = -1;
+      uint32_t off = 0;
+      // the request with before <= g < before + own
+#pragma unroll
+      for (int x = 0; x < R; x++) {
+        if (x * 32 >= a.n) break;
+        const unsigned hit = __ballot_sync(0xffffffffu, g - before[x] < own[x]);
+        if (hit) {
+          r = x * 32 + __ffs(hit) - 1;
+          off = g - __shfl_sync(0xffffffffu, before[x], __ffs(hit) - 1);
+        }
+      }
+      pc = last;
+      last.at_cost(a, sm, cap, r, off);
+    }
   } else {
     // cost before each strip of requests and in all
     const int strip = (a.n + kLine - 1) / kLine;
@@ -748,15 +812,12 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
       base += cost[x];
     }
     __syncthreads();
-    share = max((total + ctas - 1) / ctas, (uint32_t)NW);
-    const uint32_t c0 = min((unsigned long long)total, (unsigned long long)share * cta);
-    const uint32_t c1 = min(total - c0, share);
-    // c1 warp / NW without leaving 32 bits
-    auto part = [&](int w) { return c0 + c1 / NW * w + c1 % NW * w / NW; };
+    uint32_t lo, hi;
+    run_of(total, lo, hi);
 #pragma unroll 1
     for (int x = 0; x < 2; x++) {
       pc = last;
-      last.locate(a, sm, cap, part(warp + x), total, strip, lane);
+      last.locate(a, sm, cap, x ? hi : lo, total, strip, lane);
     }
   }
   auto before_last = [&](const Place<M>& x) { return x.i != last.i || x.h != last.h || x.t != last.t; };
@@ -956,14 +1017,26 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const AttnK a, int 
   pdl_launch_dependents();
   pdl_wait();
   const int cta = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
-  const int4 joint = __ldcg(reinterpret_cast<const int4*>(a.ws) + cta);
-  const int pieces = joint.z;
-  if (pieces == 0) return;
   const float2* ml = reinterpret_cast<const float2*>(a.ws + ws_stats_off(ctas)) + head;
   const float4* o = reinterpret_cast<const float4*>(a.ws + ws_o_off(ctas, a.G)) + (size_t)head * C;
   auto slot = [&](int y) { return (size_t)(y == 0 ? 2 * cta + 1 : 2 * (cta + y)) * a.G; };
-  float top = -INFINITY;
-  for (int y = tid; y < pieces; y += kJoinThreads) top = fmaxf(top, __ldcg(ml + slot(y)).x);
+  const int c = tid % C, group = tid / C, most = ctas - cta;  // no more partials than CTAs from here on
+  // The first partials are requested together with their number: what lies behind it is not used.
+  const int4 joint = __ldcg(reinterpret_cast<const int4*>(a.ws) + cta);
+  constexpr int AHEAD = 2;
+  float4 x[AHEAD];
+  float2 s[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; k++) {
+    const int y = min(group + k * GROUPS, most - 1);
+    s[k] = __ldcg(ml + slot(y));
+    x[k] = __ldcg(o + slot(y) * C + c);
+  }
+  float top = __ldcg(ml + slot(min(tid, most - 1))).x;
+  const int pieces = joint.z;
+  if (pieces == 0) return;
+  if (tid >= pieces) top = -INFINITY;
+  for (int y = tid + kJoinThreads; y < pieces; y += kJoinThreads) top = fmaxf(top, __ldcg(ml + slot(y)).x);
   top = warp_max(top);
   if ((tid & 31) == 0) tops[tid >> 5] = top;
   __syncthreads();
@@ -972,15 +1045,16 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const AttnK a, int 
   const float ref = finite_or_zero(top);
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
-  const int c = tid % C, group = tid / C;
-#pragma unroll 4
-  for (int y = group; y < pieces; y += GROUPS) {
-    const float2 s = __ldcg(ml + slot(y));
-    const float4 x = __ldcg(o + slot(y) * C + c);
+  auto add = [&](const float2& s, const float4& x) {
     const float f = pow2(s.x - ref);
     sum = fmaf(s.y, f, sum);
     v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
-  }
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; k++)
+    if (group + k * GROUPS < pieces) add(s[k], x[k]);
+#pragma unroll 4
+  for (int y = group + AHEAD * GROUPS; y < pieces; y += GROUPS) add(__ldcg(ml + slot(y)), __ldcg(o + slot(y) * C + c));
   acc[tid] = v;
   if (c == 0) sums[group] = sum;
   __syncthreads();
