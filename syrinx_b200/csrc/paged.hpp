@@ -16,6 +16,8 @@ int paged_check(const sx_paged_attention_args& a, int sms);
 cudaError_t launch_paged_plan(const sx_paged_plan_args& a, cudaStream_t st);
 cudaError_t launch_paged_append(const sx_paged_append_args& a, int sms, cudaStream_t st);
 cudaError_t launch_paged_attention(const sx_paged_attention_args& a, int sms, cudaStream_t st);
+// A (request, kv head)'s share of the attention's work beside its tiles, in tiles.
+constexpr int kPagedSegTiles = 2;
 // Most tiles and (request, kv head) pairs that the call's table can hold: they are counted in 32 bits.
 int64_t paged_attention_cost(const sx_paged_attention_args& a);
 size_t paged_attention_workspace(int G, int hd, int sms);

@@ -583,8 +583,9 @@ struct Fma {
 
 // What one (request, kv head) costs beside its tiles, in tiles: a query to load, a result to
 // write. Shares are even in tiles plus these, so that a run of very short requests is not the
-// last to finish.
-constexpr uint32_t kSegTiles = 1;
+// last to finish (64 requests of 1..4099 keys: 54.6 us with 0, 39.6 with 1, 37.1 with 2, the same
+// with 3 and 4).
+constexpr uint32_t kSegTiles = kPagedSegTiles;
 // Tiles in a warp's ring: one is computed while one is copied. With 8 warps that is 64 to 128 KB in
 // flight per SM. Three took 2.6 us longer at 168 MB: the first tiles of all warps queue up, and
 // every warp waits for them.
@@ -1073,14 +1074,17 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const AttnK a, int 
     a.lse[(size_t)joint.x * a.H + row] = total == 0.f ? -INFINITY : kLn2 * (ref + log2f(total) - lift);
 }
 
-// Lengths up to this many keys are not split over CTAs.
-constexpr int kDirectLen = 512;
+// A CTA per (request, kv head), in one launch, where they are all resident at once and have at
+// most this many tiles a warp. Measured either side of it, direct against split: 8 requests of
+// 8 kv heads of 128 in bf16, 250 keys 7.3 / 9.5 us, 500 keys 9.5 / 10.6, 1000 keys (8 tiles a
+// warp) 14.2 / 13.2; 300 requests of 1..400 keys, 16 CTAs an SM after one another, 77 / 26.
+constexpr int kDirectTiles = 4;
 
 template <class M>
 cudaError_t launch_m(AttnK a, long long bound, int sms, cudaStream_t st) {
   constexpr int TILE = 2 * M::TK * M::RB;
   const int partials = (M::NW - 1) * a.G * M::HD * 4;
-  a.direct = bound <= kDirectLen;
+  a.direct = (long long)a.n * a.Hkv <= sms && bound <= (long long)kDirectTiles * M::NW * M::TK;
   const size_t smem = (size_t)M::NW * kStages * TILE + partials;
   // the joining kernel asks for the same split of L1 and shared memory, so that it can be resident
   // (and wait) while the first one runs

@@ -128,7 +128,7 @@ int paged_check(const sx_paged_attention_args& a, int sms) {
 int64_t paged_attention_cost(const sx_paged_attention_args& a) {
   const int hd = a.cache.head_dim;
   const int keys = a.cache.dtype == SX_DTYPE_F32 ? 1024 / hd : hd == 32 ? 64 : hd == 64 ? 32 : 16;
-  const int64_t tiles = ((int64_t)a.table_width * a.cache.page_size + keys - 1) / keys + 1;
+  const int64_t tiles = ((int64_t)a.table_width * a.cache.page_size + keys - 1) / keys + kPagedSegTiles;
   const int64_t rows = (int64_t)a.n_req * a.cache.n_kv_heads;
   return rows > INT64_MAX / tiles ? INT64_MAX : rows * tiles;
 }
