@@ -144,6 +144,20 @@ int sx_model_weight_bytes(const sx_model* model, size_t* bytes_out);
 int sx_session_create(sx_model* model, int32_t max_batch, int32_t max_ctx, sx_session** out);
 int sx_session_create_ex(sx_model* model, int32_t max_batch, int32_t max_ctx, int32_t kv_dtype,
                          sx_session** out);
+/* A pooled session (no reference counterpart): the slow AR's K/V pages, of 64 positions each, are
+ * one pool of `n_pages` pages that the sequences draw from as they grow, instead of max_ctx
+ * positions set aside per sequence, so a batch of uneven sequences, or a long max_ctx, takes
+ * the memory of what is cached. Block tables, K/V appends and decode attention are the operators
+ * of include/syrinx_paged.h; the attention spreads a sequence over all SMs, which pays at long
+ * contexts, and costs three more launches per layer, which shows at short ones. All calls work
+ * as on other sessions (greedy output is the same; logits differ in the last bits, since sums
+ * are split elsewhere). A call that needs more pages than are free returns SX_E_RANGE and
+ * changes nothing; a decode loop ends early, as at max_ctx, where the pool could run out.
+ * sx_session_reset returns all pages. Tensor-parallel models: SX_E_UNSUPPORTED. */
+int sx_session_create_pool(sx_model* model, int32_t max_batch, int32_t max_ctx, int32_t kv_dtype,
+                           int32_t n_pages, sx_session** out);
+/* Pages of a pooled session that no sequence holds. */
+int sx_session_pool_free(const sx_session* s, int32_t* pages_out);
 /* Tensor-parallel sessions (no reference counterpart). Each rank writes its session's
  * SX_TP_HANDLE_BYTES-byte handle (a CUDA IPC handle of its exchange region, its GPU's UUID,
  * rank and size), the caller gathers all handles in rank order (e.g. an all-gather over

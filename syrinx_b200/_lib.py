@@ -31,6 +31,8 @@ SIGNATURES = {
     "sx_model_weight_bytes": (C.c_int, [C.c_void_p, C.POINTER(C.c_size_t)]),
     "sx_session_create": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.POINTER(C.c_void_p)]),
     "sx_session_create_ex": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_void_p)]),
+    "sx_session_create_pool": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_void_p)]),
+    "sx_session_pool_free": (C.c_int, [C.c_void_p, _i32p]),
     "sx_session_tp_handle": (C.c_int, [C.c_void_p, C.c_void_p]),
     "sx_session_tp_connect": (C.c_int, [C.c_void_p, C.c_void_p]),
     "sx_session_tp_disconnect": (C.c_int, [C.c_void_p]),

@@ -210,6 +210,34 @@ int sx_session_create_ex(sx_model* model, int32_t max_batch, int32_t max_ctx, in
   })
 }
 
+int sx_session_create_pool(sx_model* model, int32_t max_batch, int32_t max_ctx, int32_t kv_dtype, int32_t n_pages,
+                           sx_session** out) {
+  SX_GUARD({
+    if (!model) {
+      set_error("null model");
+      return SX_E_INVALID;
+    }
+    if (n_pages < 1) {
+      set_error("sx_session_create_pool: n_pages must be positive");
+      return SX_E_INVALID;
+    }
+    int rc = use_device(model);
+    if (rc) return rc;
+    return session_create(model, max_batch, max_ctx, kv_dtype, out, n_pages);
+  })
+}
+
+int sx_session_pool_free(const sx_session* s, int32_t* pages_out) {
+  if (!s || !pages_out || !s->pool) {
+    set_error("sx_session_pool_free: null argument, or not a pooled session");
+    return SX_E_INVALID;
+  }
+  int64_t held = 0;
+  for (int len : s->pool_high) held += (len + kPage - 1) / kPage;
+  *pages_out = (int32_t)(s->n_pages - held);
+  return SX_OK;
+}
+
 int sx_session_reset(sx_session* s) {
   SX_GUARD({
     if (!s) {

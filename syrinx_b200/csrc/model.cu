@@ -16,6 +16,7 @@
 #include <cstring>
 #include <cstdlib>
 
+#include "paged.hpp"
 #include "sx_internal.hpp"
 
 namespace sx {
@@ -443,7 +444,46 @@ void model_destroy(sx_model* m) {
 // ---------------------------------------------------------------------------------------
 // sessions
 // ---------------------------------------------------------------------------------------
-int session_create(sx_model* m, int max_batch, int max_ctx, int kv_dtype, sx_session** out) {
+namespace {
+
+// Every page of a pooled session free, every sequence empty (ordered on the session's stream).
+int pool_clear(sx_session* s) {
+  std::vector<int> ids(s->n_pages), zeros(s->max_batch, 0);
+  for (int i = 0; i < s->n_pages; i++) ids[i] = s->n_pages - 1 - i;  // page 0 on top of the stack
+  SX_CU(cudaMemcpyAsync(s->free_pages, ids.data(), ids.size() * 4, cudaMemcpyHostToDevice, s->st));
+  SX_CU(cudaMemcpyAsync(s->n_free, &s->n_pages, 4, cudaMemcpyHostToDevice, s->st));
+  SX_CU(cudaMemcpyAsync(s->pool_len, zeros.data(), zeros.size() * 4, cudaMemcpyHostToDevice, s->st));
+  SX_CU(cudaStreamSynchronize(s->st));
+  std::fill(s->pool_high.begin(), s->pool_high.end(), 0);
+  return SX_OK;
+}
+
+// Pages the session would hold with sequence i at targets(i) positions at least.
+template <class F>
+int64_t pool_pages_at(const sx_session* s, F&& targets) {
+  int64_t pages = 0;
+  for (int i = 0; i < s->max_batch; i++) pages += (std::max(s->pool_high[i], targets(i)) + kPage - 1) / kPage;
+  return pages;
+}
+
+// Notes that sequence i is about to grow to targets(i) positions; SX_E_RANGE, and nothing noted,
+// if the pool does not hold them. Every step that writes K/V passes here before it is enqueued,
+// so the device never runs out of pages.
+template <class F>
+int pool_reserve(sx_session* s, F&& targets) {
+  if (!s->pool) return SX_OK;
+  const int64_t pages = pool_pages_at(s, targets);
+  if (pages > s->n_pages) {
+    set_error("page pool exhausted: " + std::to_string(pages) + " pages needed of " + std::to_string(s->n_pages));
+    return SX_E_RANGE;
+  }
+  for (int i = 0; i < s->max_batch; i++) s->pool_high[i] = std::max(s->pool_high[i], targets(i));
+  return SX_OK;
+}
+
+}  // namespace
+
+int session_create(sx_model* m, int max_batch, int max_ctx, int kv_dtype, sx_session** out, int pool_pages) {
   if (!m || !out || max_batch < 1 || max_batch > kMaxTok || max_ctx < 1) {
     set_error("sx_session_create: max_batch must be 1..8 and max_ctx >= 1");
     return SX_E_INVALID;
@@ -451,6 +491,14 @@ int session_create(sx_model* m, int max_batch, int max_ctx, int kv_dtype, sx_ses
   if (kv_dtype != SX_DTYPE_F32 && kv_dtype != SX_DTYPE_BF16) {
     set_error("sx_session_create: kv_dtype must be SX_DTYPE_F32 or SX_DTYPE_BF16");
     return SX_E_UNSUPPORTED;
+  }
+  if (pool_pages && m->tp_size > 1) {
+    set_error("sx_session_create_pool: tensor-parallel models keep sx_session_create");
+    return SX_E_UNSUPPORTED;
+  }
+  if ((int64_t)pool_pages * kPage > INT32_MAX) {
+    set_error("sx_session_create_pool: the pool must hold fewer than 2^31 positions");
+    return SX_E_RANGE;
   }
   SX_CU(cudaSetDevice(m->device));
   const sx_model_desc& d = m->d;
@@ -473,16 +521,36 @@ int session_create(sx_model* m, int max_batch, int max_ctx, int kv_dtype, sx_ses
   s->st = s->own_st;
   const auto& sl = d.slow;
   s->pages_per_seq = (max_ctx + kPage - 1) / kPage;
-  s->n_pages = max_batch * s->pages_per_seq;
+  s->pool = pool_pages > 0;
+  s->n_pages = s->pool ? pool_pages : max_batch * s->pages_per_seq;
   s->kv_layer_elems = (size_t)2 * s->n_pages * sl.n_local_heads * kPage * sl.head_dim;
   int rc;
   if ((rc = dalloc(s->allocs, &s->kv, s->kv_layer_elems * sl.n_layer * s->kv_elem))) return fail(rc);
-  if ((rc = dalloc(s->allocs, &s->page_table, (size_t)s->n_pages))) return fail(rc);
+  const int table_entries = max_batch * s->pages_per_seq;
+  if ((rc = dalloc(s->allocs, &s->page_table, (size_t)table_entries))) return fail(rc);
   {
-    std::vector<int> pt(s->n_pages);
-    for (int i = 0; i < s->n_pages; i++) pt[i] = i;  // sequence b owns pages [b*pps, (b+1)*pps)
+    std::vector<int> pt(table_entries, 0);
+    if (!s->pool)
+      for (int i = 0; i < table_entries; i++) pt[i] = i;  // sequence b owns pages [b*pps, (b+1)*pps)
     if (cudaMemcpy(s->page_table, pt.data(), pt.size() * 4, cudaMemcpyHostToDevice) != cudaSuccess)
       return fail(SX_E_CUDA);
+  }
+  if (s->pool) {
+    const size_t angles = (size_t)max_ctx * (sl.head_dim / 2);
+    s->pool_high.assign(max_batch, 0);
+    s->pool_ws_bytes = paged_attention_workspace(sl.n_head / sl.n_local_heads, sl.head_dim, paged_sms(m->device));
+    if ((rc = dalloc(s->allocs, &s->free_pages, (size_t)s->n_pages)) || (rc = dalloc(s->allocs, &s->n_free, 1)) ||
+        (rc = dalloc(s->allocs, &s->pool_len, max_batch)) || (rc = dalloc(s->allocs, &s->pool_delta, max_batch)) ||
+        (rc = dalloc(s->allocs, &s->plan_status, 4)) || (rc = dalloc(s->allocs, &s->pool_slots, kMaxPrefillTok)) ||
+        (rc = dalloc(s->allocs, &s->att_len, kMaxPrefillTok)) ||
+        (rc = dalloc(s->allocs, &s->pool_q, (size_t)kMaxTok * sl.n_head * sl.head_dim)) ||
+        (rc = dalloc(s->allocs, &s->rope_cos, angles)) || (rc = dalloc(s->allocs, &s->rope_sin, angles)) ||
+        (rc = dalloc(s->allocs, &s->pool_ws, s->pool_ws_bytes)) || (rc = pool_clear(s)))
+      return fail(rc);
+    if (launch_rope_table(m->inv_slow, sl.head_dim / 2, max_ctx, s->rope_cos, s->rope_sin, s->st) != cudaSuccess) {
+      set_error("rotation tables: launch failed");
+      return fail(SX_E_CUDA);
+    }
   }
   const int C = d.num_codebooks;
   const bool has_fast = d.fast.n_layer > 0;
@@ -719,6 +787,10 @@ int session_tp_set_timeout(sx_session* s, int64_t timeout_ns) {
 }
 
 int session_reset(sx_session* s) {
+  if (s->pool) {
+    SX_CU(cudaSetDevice(s->m->device));
+    SX_RC(pool_clear(s));
+  }
   std::fill(s->len.begin(), s->len.end(), 0);
   std::fill(s->synthetic_len.begin(), s->synthetic_len.end(), 0);
   return SX_OK;
@@ -779,7 +851,7 @@ bool stack_args(sx_session* s, bool fast, int M, float* resid, const int* tok_se
                 int const_pos, StackArgs* out) {
   sx_model* m = s->m;
   const StackLayer* layers = fast ? m->fast_stack : m->slow_stack;
-  if (!layers || M > kMaxTok || m->tp_size > 1) return false;
+  if (!layers || M > kMaxTok || m->tp_size > 1 || (s->pool && !fast)) return false;
   const sx_transformer_desc& td = fast ? m->d.fast : m->d.slow;
   const int sms = num_sms_of(m->device);
   StackArgs a;
@@ -891,6 +963,97 @@ int glu_fold_chunks(const sx_session* s, const DevLayer& L, int M) {
   return nc <= kQkvChunks ? nc : 0;
 }
 
+// Pages for a step's tokens in a pooled session: block tables for the grown lengths, then the
+// tokens' slots and attention lengths. Once per step, before the first layer.
+int pool_step(sx_session* s, int M, const int* tok_seq, const int* tok_pos) {
+  PoolArgs p;
+  p.tok_seq = tok_seq;
+  p.tok_pos = tok_pos;
+  p.M = M;
+  p.batch = s->max_batch;
+  p.pages_per_seq = s->pages_per_seq;
+  p.lens = s->pool_len;
+  p.delta = s->pool_delta;
+  p.table = s->page_table;
+  p.status = s->plan_status;
+  p.slots = s->pool_slots;
+  p.att_len = s->att_len;
+  p.err = s->err;
+  SX_CU(launch_pool_begin(p, s->st));
+  sx_paged_plan_args a{};
+  a.lens_in = a.lens_out = s->pool_len;
+  a.delta = s->pool_delta;
+  a.n_free_in = a.n_free_out = s->n_free;
+  a.table = s->page_table;
+  a.free_pages = s->free_pages;
+  a.status = s->plan_status;
+  a.table_stride = a.table_width = s->pages_per_seq;
+  a.n_req = s->max_batch;
+  a.n_pages = s->n_pages;
+  a.page_size = kPage;
+  SX_RC(paged_check(a));
+  SX_CU(launch_paged_plan(a, s->st));
+  SX_CU(launch_pool_slots(p, s->st));
+  return SX_OK;
+}
+
+// A slow layer's K/V append (and, in decode, its normed and rotated queries and its attention) in
+// a pooled session. `a` is the layer as the static session's kernels take it.
+int pool_attention(sx_session* s, const AttnArgs& a, bool append) {
+  const int sms = num_sms_of(s->m->device);
+  sx_paged_append_args w{};
+  w.cache.k = a.kbase;
+  w.cache.v = a.vbase;
+  w.cache.token_stride = a.hd;
+  w.cache.head_stride = (int64_t)kPage * a.hd;
+  w.cache.page_stride = (int64_t)a.Hkv * kPage * a.hd;
+  w.cache.dtype = a.kv_f32 ? SX_DTYPE_F32 : SX_DTYPE_BF16;
+  w.cache.n_pages = s->n_pages;
+  w.cache.page_size = kPage;
+  w.cache.n_kv_heads = a.Hkv;
+  w.cache.head_dim = a.hd;
+  w.x = a.qkv;
+  w.x_stride = (int64_t)(a.H + 2 * a.Hkv) * a.hd;
+  w.x_dtype = SX_DTYPE_F32;
+  w.q_out = append ? s->pool_q : nullptr;  // the prefill kernel norms and rotates its own queries
+  w.q_stride = (int64_t)a.H * a.hd;
+  w.slots = s->pool_slots;
+  w.positions = a.tok_pos;
+  w.cos = s->rope_cos;
+  w.sin = s->rope_sin;
+  w.n_positions = s->max_ctx;
+  w.q_norm = a.qn;
+  w.k_norm = a.kn;
+  w.eps = a.eps;
+  w.n_rows = a.M;
+  w.n_heads = a.H;
+  w.interleaved = a.interleaved;
+  SX_RC(paged_check(w));
+  SX_CU(launch_paged_append(w, sms, s->st));
+  if (!append) {
+    SX_CU(launch_attention_prefill(a, s->st));
+    return SX_OK;
+  }
+  sx_paged_attention_args t{};
+  t.cache = w.cache;
+  t.q = s->pool_q;
+  t.out = a.out;
+  t.q_stride = t.out_stride = w.q_stride;
+  t.table = s->page_table;  // token t of a decode step is sequence t
+  t.table_stride = t.table_width = s->pages_per_seq;
+  t.lens = s->att_len;
+  t.workspace = s->pool_ws;
+  t.workspace_bytes = s->pool_ws_bytes;
+  t.n_req = a.M;
+  t.n_heads = a.H;
+  t.q_dtype = SX_DTYPE_F32;
+  t.max_len = s->max_ctx;
+  t.scale = a.scale;
+  SX_RC(paged_check(t, sms));
+  SX_CU(launch_paged_attention(t, sms, s->st));
+  return SX_OK;
+}
+
 // One transformer stack over M tokens. resid [M][dim] is updated in place.
 int run_stack(sx_session* s, bool fast, int M, float* resid, const int* tok_seq, const int* tok_pos,
               int const_pos, bool append) {
@@ -903,6 +1066,8 @@ int run_stack(sx_session* s, bool fast, int M, float* resid, const int* tok_seq,
   const int qkv_w = (td.n_head + 2 * td.n_local_heads) * td.head_dim;
   const size_t layer_elems = fast ? s->fkv_layer_elems : s->kv_layer_elems;
   const size_t half = layer_elems / 2;
+  const bool pool = s->pool && !fast;
+  if (pool) SX_RC(pool_step(s, M, tok_seq, tok_pos));
   for (size_t l = 0; l < layers.size(); l++) {
     const DevLayer& L = layers[l];
     GemvArgs g;
@@ -915,7 +1080,7 @@ int run_stack(sx_session* s, bool fast, int M, float* resid, const int* tok_seq,
     g.ldy = qkv_w;
     g.M = M;
     g.n_range = qkv_w;
-    const int fold_nc = qkv_fold_chunks(L.wqkv, M, append);
+    const int fold_nc = pool ? 0 : qkv_fold_chunks(L.wqkv, M, append);
     SX_RC(gemv(g, fold_nc ? EPI_NONE : EPI_STORE, s));
 
     AttnArgs a;
@@ -950,7 +1115,9 @@ int run_stack(sx_session* s, bool fast, int M, float* resid, const int* tok_seq,
     a.n_split = fast ? 1 : n_split_for(s, M, td.n_local_heads);
     a.append = append ? 1 : 0;
     a.M = M;
-    if (append) {
+    if (pool) {
+      SX_RC(pool_attention(s, a, append));
+    } else if (append) {
       SX_CU(launch_attention(a, s->st));
     } else {  // a prompt chunk of one sequence: its K/V first, then the tiled prefill kernel
       SX_CU(launch_kv_append(a, s->st));
@@ -1019,6 +1186,10 @@ int check_err(sx_session* s) {
   }
   SX_CU(cudaMemsetAsync(s->err, 0, 4, s->st));
   SX_CU(cudaStreamSynchronize(s->st));
+  if (e == 4) {
+    set_error("the page pool could not give a sequence its pages (device error flag)");
+    return SX_E_DEVICE;
+  }
   if (e == 2) {
     set_error("a kernel's bounded pipeline wait timed out (device error flag)");
     return SX_E_DEVICE;
@@ -1048,7 +1219,7 @@ EmbedArgs embed_args(sx_session* s) {
 namespace {
 // Seeded pseudo-random K/V values in [-1, 1) for positions [0, len) of one sequence, every
 // slow layer (SplitMix64 of seed and the element's coordinates).
-__global__ void k_fill_kv(uint8_t* kv, size_t layer_elems, int n_layer, int first_page, int Hkv, int hd, int len,
+__global__ void k_fill_kv(uint8_t* kv, size_t layer_elems, int n_layer, const int* pages, int Hkv, int hd, int len,
                           int kv_f32, uint64_t seed) {
   const size_t half = layer_elems / 2;
   const size_t per_layer = (size_t)2 * len * Hkv * hd;
@@ -1068,7 +1239,7 @@ __global__ void k_fill_kv(uint8_t* kv, size_t layer_elems, int n_layer, int firs
     z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
     z ^= z >> 31;
     const float v = (float)(z >> 40) * (1.0f / 8388608.0f) - 1.0f;
-    const size_t page = (size_t)first_page + pos / kPage;
+    const size_t page = (size_t)pages[pos / kPage];
     const size_t e = (size_t)l * layer_elems + which * half + ((page * Hkv + h) * kPage + pos % kPage) * hd + d;
     if (kv_f32)
       reinterpret_cast<float*>(kv)[e] = v;
@@ -1092,7 +1263,13 @@ int fill_kv_synthetic(sx_session* s, int seq, int len, uint64_t seed) {
   }
   const auto& sl = s->m->d.slow;
   (void)cudaGetLastError();
-  k_fill_kv<<<1184, 256, 0, s->st>>>(s->kv, s->kv_layer_elems, sl.n_layer, seq * s->pages_per_seq, sl.n_local_heads,
+  if (s->pool) {
+    SX_RC(pool_reserve(s, [&](int i) { return i == seq ? len : 0; }));
+    SX_RC(upload_tokens(s, s->ptok_seq, s->ptok_pos, {seq}, {len - 1}));
+    SX_RC(pool_step(s, 1, s->ptok_seq, s->ptok_pos));
+  }
+  k_fill_kv<<<1184, 256, 0, s->st>>>(s->kv, s->kv_layer_elems, sl.n_layer, s->page_table + (size_t)seq * s->pages_per_seq,
+                                     sl.n_local_heads,
                                      sl.head_dim, len, s->kv_f32, seed);
   SX_CU(cudaGetLastError());
   SX_CU(cudaStreamSynchronize(s->st));
@@ -1112,6 +1289,7 @@ int prefill_seq(sx_session* s, int seq, const uint32_t* prompt, int T) {
     set_error("prefill: prompt exceeds the session's max_ctx");
     return SX_E_RANGE;
   }
+  SX_RC(pool_reserve(s, [&](int i) { return i == seq ? s->len[i] + T : 0; }));
   SX_CU(cudaMemcpyAsync(s->prompt, prompt, (size_t)rows * T * 4, cudaMemcpyHostToDevice, s->st));
   const int base = s->len[seq];
   int last_M = 0;
@@ -1151,6 +1329,7 @@ int prefill_seq_embeds(sx_session* s, int seq, const float* embeds, int T) {
     set_error("lm_step_embeds: input exceeds the session's max_ctx");
     return SX_E_RANGE;
   }
+  SX_RC(pool_reserve(s, [&](int i) { return i == seq ? s->len[i] + T : 0; }));
   const int base = s->len[seq];
   int last_M = 0;
   for (int c0 = 0; c0 < T; c0 += kMaxPrefillTok) {
@@ -1192,6 +1371,7 @@ int slow_step_enqueue(sx_session* s, const int* seqs, const uint32_t* frames, in
     ts[i] = i;
     tp[i] = s->len[i];
   }
+  SX_RC(pool_reserve(s, [&](int i) { return i < n ? s->len[i] + 1 : 0; }));
   SX_CU(cudaMemcpyAsync(s->frames, frames, (size_t)n * width * 4, cudaMemcpyHostToDevice, s->st));
   SX_RC(upload_tokens(s, s->tok_seq, s->tok_pos, ts, tp));
   EmbedArgs e = embed_args(s);
@@ -1618,6 +1798,20 @@ int run_frames(sx_session* s, int n, int n_frames, int mask_stop, bool sampled, 
   // each frame's trailing slow step writes position len + f
   n_frames = std::min(n_frames, s->max_ctx - max_len);
   n_frames = std::min(n_frames, s->ring_frames);
+  if (s->pool) {
+    // as many frames as the pool has pages for if no sequence stops
+    auto after = [&](int f) { return [s, n, f](int i) { return i < n ? s->len[i] + f : 0; }; };
+    int lo = 0, hi = std::max(0, n_frames);
+    while (lo < hi) {
+      const int mid = lo + (hi - lo + 1) / 2;
+      if (pool_pages_at(s, after(mid)) <= s->n_pages)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    n_frames = std::min(n_frames, lo);
+    SX_RC(pool_reserve(s, after(n_frames)));
+  }
   std::vector<int> ts(n), tp(n), zeros(n, 0);
   for (int i = 0; i < n; i++) {
     ts[i] = i;
@@ -1640,7 +1834,9 @@ int run_frames(sx_session* s, int n, int n_frames, int mask_stop, bool sampled, 
     gg = &s->graphs.back();
   }
   for (int f = 0; f < n_frames; f++) SX_CU(cudaGraphLaunch(gg->exec, s->st));
-  std::vector<int> counts(n), lens(n);
+  std::vector<int> counts(n), lens(n), held(s->max_batch);
+  if (s->pool)
+    SX_CU(cudaMemcpyAsync(held.data(), s->pool_len, held.size() * 4, cudaMemcpyDeviceToHost, s->st));
   SX_CU(cudaMemcpyAsync(counts.data(), s->frame_count, n * 4, cudaMemcpyDeviceToHost, s->st));
   SX_CU(cudaMemcpyAsync(lens.data(), s->seq_len, n * 4, cudaMemcpyDeviceToHost, s->st));
   std::vector<uint32_t> ring((size_t)std::max(1, n_frames) * s->max_batch * width);
@@ -1648,6 +1844,7 @@ int run_frames(sx_session* s, int n, int n_frames, int mask_stop, bool sampled, 
     SX_CU(cudaMemcpyAsync(ring.data(), s->ring, (size_t)n_frames * s->max_batch * width * 4,
                           cudaMemcpyDeviceToHost, s->st));
   SX_CU(cudaStreamSynchronize(s->st));
+  if (s->pool) s->pool_high = held;
   for (int i = 0; i < n; i++) {
     const int c = std::min(counts[i], n_frames);
     if (n_frames_out) n_frames_out[i] = c;
@@ -1803,6 +2000,7 @@ int frame_step_greedy(sx_session* s, const uint32_t* frame_in, int mask_stop, ui
       set_error("frame_step: context exceeds the session's max_ctx");
       return SX_E_RANGE;
     }
+    SX_RC(pool_reserve(s, [&](int i) { return i == 0 ? s->len[0] + 1 : 0; }));
     // the frame and its position go to device memory; the captured frame graph reads them
     const std::vector<int> ts{0}, tp{s->len[0]};
     SX_CU(cudaMemcpyAsync(s->frames, frame_in, (size_t)width * 4, cudaMemcpyHostToDevice, s->st));

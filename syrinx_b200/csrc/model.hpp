@@ -100,6 +100,22 @@ struct sx_session {
   std::vector<int> len;  // host mirror of per-sequence cache lengths
   std::vector<int> synthetic_len;  // positions filled by fill_kv_synthetic (a prefill may follow)
   bool device_len_dirty = false;  // device seq_len advanced by a graph loop
+  // pooled session: the slow AR's pages come from one pool (sx_paged_plan), its decode attention
+  // and K/V appends are the paged operators
+  bool pool = false;
+  int* free_pages = nullptr;   // [n_pages] the stack of free pages
+  int* n_free = nullptr;       // [1]
+  int* pool_len = nullptr;     // [max_batch] positions with pages
+  int* pool_delta = nullptr;   // [max_batch]
+  int* plan_status = nullptr;  // [4]
+  int* pool_slots = nullptr;   // [kMaxPrefillTok]
+  int* att_len = nullptr;      // [kMaxPrefillTok]
+  float* pool_q = nullptr;     // [kMaxTok][H hd] normed, rotated queries
+  float* rope_cos = nullptr;   // [max_ctx][hd / 2]
+  float* rope_sin = nullptr;
+  uint8_t* pool_ws = nullptr;
+  size_t pool_ws_bytes = 0;
+  std::vector<int> pool_high;  // host mirror of pool_len (never below it)
   std::vector<GreedyGraph> graphs;
   std::vector<void*> allocs;
 };
@@ -117,7 +133,8 @@ int fill_kv_synthetic(sx_session* s, int seq, int len, uint64_t seed);
 int decode_sample(sx_session* s, int n_frames, uint64_t seed, const sx_sampling_params* p, uint32_t* frames_out,
                   int* n_frames_out);
 void model_destroy(sx_model* m);
-int session_create(sx_model* m, int max_batch, int max_ctx, int kv_dtype, sx_session** out);
+// pool_pages > 0: a pooled session of that many pages
+int session_create(sx_model* m, int max_batch, int max_ctx, int kv_dtype, sx_session** out, int pool_pages = 0);
 void session_destroy(sx_session* s);
 int session_reset(sx_session* s);
 int sync_lengths(sx_session* s);

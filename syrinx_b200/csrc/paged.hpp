@@ -22,6 +22,26 @@ constexpr int kPagedSegTiles = 2;
 int64_t paged_attention_cost(const sx_paged_attention_args& a);
 size_t paged_attention_workspace(int G, int hd, int sms);
 
+// ---- pooled sessions (pool.cu) --------------------------------------------------------------
+struct PoolArgs {
+  const int* tok_seq = nullptr;  // [M] sequence and position of each token of the step
+  const int* tok_pos = nullptr;
+  int M = 0;
+  int batch = 0;          // sequences of the session
+  int pages_per_seq = 0;  // width of the table
+  const int* lens = nullptr;    // [batch] positions each sequence holds pages for
+  int* delta = nullptr;         // [batch] what the step adds to them
+  const int* table = nullptr;   // [batch][pages_per_seq]
+  const int* status = nullptr;  // of sx_paged_plan
+  int* slots = nullptr;         // [M]
+  int* att_len = nullptr;       // [M]
+  int* err = nullptr;           // the session's device error flag (4: the pool could not grow)
+};
+cudaError_t launch_pool_begin(const PoolArgs& a, cudaStream_t st);
+cudaError_t launch_pool_slots(const PoolArgs& a, cudaStream_t st);
+// cos / sin [n_pos][half] of (float)position * inv_freq, rounded to f32 before the functions
+cudaError_t launch_rope_table(const float* inv_freq, int half, int n_pos, float* cosv, float* sinv, cudaStream_t st);
+
 int paged_sms(int device);  // SMs of a device (0: there is no such device)
 
 }  // namespace sx

@@ -82,17 +82,30 @@ class SlowStep:
 class B200DualAr:
     """`DualArBackend` over the B200 kernels, one session of up to `max_batch` sequences."""
 
-    def __init__(self, model: Model, max_ctx: int, max_batch: int = 1, kv_dtype: int = SX_DTYPE_F32):
+    def __init__(self, model: Model, max_ctx: int, max_batch: int = 1, kv_dtype: int = SX_DTYPE_F32,
+                 pool_pages: int = 0):
         """kv_dtype SX_DTYPE_F32 (default, the reference CPU cache: token-exact greedy output)
-        or SX_DTYPE_BF16 (half the KV bytes, for long contexts and batched decode)."""
+        or SX_DTYPE_BF16 (half the KV bytes, for long contexts and batched decode).
+        pool_pages > 0: the sequences draw their KV pages (64 positions each) from one pool of
+        that many, instead of max_ctx positions set aside for each (sx_session_create_pool)."""
         self.model = model
         self.cfg = model.cfg
         self.max_ctx = max_ctx
         self.max_batch = max_batch
         self.kv_dtype = kv_dtype
         self.handle = C.c_void_p()
-        _lib.check(_lib.lib().sx_session_create_ex(model.handle, max_batch, max_ctx, kv_dtype,
-                                                   C.byref(self.handle)))
+        if pool_pages:
+            _lib.check(_lib.lib().sx_session_create_pool(model.handle, max_batch, max_ctx, kv_dtype, pool_pages,
+                                                         C.byref(self.handle)))
+        else:
+            _lib.check(_lib.lib().sx_session_create_ex(model.handle, max_batch, max_ctx, kv_dtype,
+                                                       C.byref(self.handle)))
+
+    def pool_free(self) -> int:
+        """Pages of a pooled session that no sequence holds."""
+        n = C.c_int32()
+        _lib.check(_lib.lib().sx_session_pool_free(self.handle, C.byref(n)))
+        return n.value
 
     # -- tensor parallelism ----------------------------------------------------------------
     def tp_handle(self) -> bytes:
