@@ -31,7 +31,7 @@ namespace sx {
 namespace {
 
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanCtas = 8;  // of a cluster
+constexpr int kPlanCtas = 16;  // of a cluster, more than the portable 8
 constexpr int kKept = 4;      // page moves a thread keeps from the check to the write
 
 __device__ __forceinline__ int pages_of(long long len, int shift) {
@@ -134,8 +134,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const sx_paged_plan
   const int tid = threadIdx.x, n = a.n_req;
   const int all = ctas * kPlanThreads, me = rank * kPlanThreads + tid;
   int* start = dyn;          // [n + 1] exclusive sums of the new tokens
-  int* gs = start + n + 1;   // [n] of the pages given back
-  int* ts = gs + n;          // [n] of the pages taken
+  int* gs = start + n + 1;   // [n + 1] of the pages given back
+  int* ts = gs + n + 1;      // [n] of the pages taken
   int* len = ts + n;         // [n] old lengths
   const int shift = __ffs(a.page_size) - 1;
   pdl_launch_dependents();
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const sx_paged_plan
       v[1] += max(0, h - m);
       v[2] += max(0, m - h);
     }
-    if (tid == 0) start[n] = (int)sum[0];
+    if (tid == 0) start[n] = (int)sum[0], gs[n] = (int)sum[1];
     __syncthreads();
   }
   // every CTA has come to the same err, G and T here
@@ -185,8 +185,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const sx_paged_plan
   // entry k of the pushes: a page its row no longer needs
   auto pushed = [&](int k) {
     const int r = last_not_above(gs, n, k);
-    const int m = pages_of(max(0ll, (long long)len[r] + ld_cg(a.delta + r)), shift);
-    return ld_cg(a.table + (size_t)r * a.table_stride + m + (k - gs[r]));
+    // the row keeps its pages but for the ones it gives: the last gs[r + 1] - gs[r]
+    return ld_cg(a.table + (size_t)r * a.table_stride + pages_of(len[r], shift) - (gs[r + 1] - k));
   };
   auto moved = [&](int k) {
     if (k >= T) return pushed(k - T);
@@ -254,8 +254,9 @@ cudaError_t launch_paged_plan(const sx_paged_plan_args& a, cudaStream_t st) {
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
   if (device >= 64 || !(ready.load(std::memory_order_acquire) >> device & 1)) {
-    constexpr int most = (4 * SX_PAGED_MAX_REQUESTS + 1) * 4;
-    if ((e = cudaFuncSetAttribute(k_paged_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) != cudaSuccess)
+    constexpr int most = (4 * SX_PAGED_MAX_REQUESTS + 2) * 4;
+    if ((e = cudaFuncSetAttribute(k_paged_plan, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute(k_paged_plan, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess)
       return e;
     if (device < 64) ready.fetch_or(1ull << device, std::memory_order_release);
   }
@@ -263,7 +264,7 @@ cudaError_t launch_paged_plan(const sx_paged_plan_args& a, cudaStream_t st) {
   const bool small = (long long)a.n_req * a.table_width <= kKept * kPlanThreads && a.max_tokens <= 4 * kPlanThreads;
   const unsigned ctas = small ? 1 : kPlanCtas;
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = launch_cfg(dim3(ctas), dim3(kPlanThreads), (size_t)(4 * a.n_req + 1) * 4, st, attr);
+  cudaLaunchConfig_t cfg = launch_cfg(dim3(ctas), dim3(kPlanThreads), (size_t)(4 * a.n_req + 2) * 4, st, attr);
   if (ctas > 1) {
     cudaLaunchAttribute& c = attr[cfg.numAttrs++];
     c.id = cudaLaunchAttributeClusterDimension;
