@@ -61,8 +61,8 @@ typedef struct sx_paged_cache {
  * status[0] is SX_OK or why nothing was changed: SX_E_RANGE (too few free pages, more than
  * max_tokens new tokens, a row longer than table_width pages) or SX_E_INVALID (a negative
  * length, a stack larger than n_pages, a page id outside the pool). In that case the lengths,
- * the stack and the table stay as they were and every slot, request and position is -1, so
- * that a following append writes nothing. status[1 .. 3]: new tokens, pages popped, pages
+ * the stack and the table stay as they were, every slot, request and position is -1, so that a
+ * following append writes nothing, and `starts` is 0. status[1 .. 3]: new tokens, pages popped, pages
  * free afterwards.
  */
 typedef struct sx_paged_plan_args {
@@ -98,7 +98,7 @@ int sx_paged_plan(const sx_paged_plan_args* args, int32_t device, void* cuda_str
  * (interleaved) or (i, i + head_dim / 2) by the angle whose cosine and sine stand in row
  * positions[j] of `cos` / `sin` (null: none). Query heads go to q_out (null: they are
  * dropped), keys and values into the cache at slots[j]. A row with slot -1 writes nothing.
- * Arithmetic is f32. Rows must not share a slot.
+ * Arithmetic is f32. Rows must not share a slot. q_out may be the query part of x itself.
  *
  * A slot outside the cache or a position outside the tables writes nothing for that row and
  * sets *status (nullable) to SX_E_RANGE; status is not written otherwise.
@@ -136,8 +136,8 @@ int sx_paged_append(const sx_paged_append_args* args, int32_t device, void* cuda
  * A length beyond table_width pages is cut to it, and a page id outside the cache reads as
  * zeros; either sets *status (nullable) to SX_E_RANGE, which is not written otherwise.
  *
- * The key axis of all requests is cut into even shares for the GPU's SMs; partial results
- * pass through `workspace`, whose content means nothing before and after the call. Calls that
+ * The key axis of all requests is cut into even shares for the GPU's SMs (so the last bits of
+ * a result depend on the lengths of all of them); partial results pass through `workspace`, whose content means nothing before and after the call. Calls that
  * may run at the same time (on two streams, or two captured graphs) need a workspace each.
  */
 typedef struct sx_paged_attention_args {
@@ -153,7 +153,7 @@ typedef struct sx_paged_attention_args {
   int64_t q_stride, out_stride; /* elements, multiples of 16 bytes */
   int64_t table_stride;
   int32_t table_width;
-  int32_t n_req;   /* 0: nothing is done */
+  int32_t n_req;   /* 0: nothing is done; n_req x kv heads x tiles of a row below 2^32 */
   int32_t n_heads; /* n_kv_heads x 1 .. 16 (1 .. 8 at head_dim 256) */
   int32_t q_dtype; /* SX_DTYPE_F32, or the cache's type */
   int32_t max_len; /* what no length exceeds, as far as the host knows (0: table_width pages);

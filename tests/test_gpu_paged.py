@@ -177,6 +177,37 @@ def test_attend_many_uneven_requests(paged, qt, ct):
     assert_attends(paged, q, k, v, table, lens, 16, "nhd")
 
 
+@pytest.mark.parametrize("n", [32, 33, 127, 128, 129, 512, 513, 1025])
+@pytest.mark.parametrize("qt,ct,hd", [("f32", "f32", 64), ("bf16", "bf16", 128)])
+def test_attend_request_counts(paged, qt, ct, hd, n):
+    """Either side of the counts at which the requests are summed up in another way."""
+    lens = [(37 * i * i + 11 * i) % 290 if i % 7 else 0 for i in range(n)]
+    lens[n // 2] = 3000
+    k, v, table = filled(lens, 2, 16, hd, DT[ct], "hnd", n)
+    q = torch.randn((n, 4, hd), generator=gen(n), device="cuda").to(DT[qt])
+    assert_attends(paged, q, k, v, table, lens, 16, "hnd")
+
+
+def test_attend_on_two_streams_at_once(paged):
+    """Eager calls on two streams take a workspace each from the allocator."""
+    lens = [5000, 300, 2000]
+    k, v, table = filled(lens, 2, 16, 128, torch.bfloat16, "hnd", 5)
+    d = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    qs = [torch.randn((3, 8, 128), generator=gen(s), device="cuda").bfloat16() for s in range(2)]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(30):
+        for s in range(2):
+            with torch.cuda.stream(streams[s]):
+                outs[s].append(paged.attend(qs[s], k, v, table, d))
+    torch.cuda.synchronize()
+    for s in range(2):
+        want, _, tol, _ = ref_attend(qs[s], k, v, table, lens, 128 ** -0.5, 16, "hnd")
+        assert ((outs[s][0].double() - want).abs() <= tol).all()
+        assert all(torch.equal(o, outs[s][0]) for o in outs[s])
+
+
 def test_attend_thousands_of_requests(paged):
     lens = [(7 * i) % 5 for i in range(5000)]
     k, v, table = filled([0] * 5000, 1, 8, 32, torch.float32, "hnd", 1)
@@ -475,6 +506,25 @@ def test_append(paged, xt, ct, H, hkv, hd, norm, rot, il):
 @pytest.mark.parametrize("xt,ct", TYPES)
 def test_append_many_rows(paged, xt, ct):
     assert_appends(paged, 3001, 5, 16, 8, 64, 32, xt, ct, "nhd", (1, 1), 1, False, 3, strided=True)
+
+
+@pytest.mark.parametrize("T", [3, 4000])
+@pytest.mark.parametrize("il", [True, False])
+def test_append_queries_in_place(paged, T, il):
+    """The query part of x may be its own output."""
+    H, hkv, hd = 4, 2, 64
+    x = torch.randn((T, 8 * 64), generator=gen(1), device="cuda")
+    cos, sin = rope(100, hd)
+    pos = torch.arange(T, device="cuda", dtype=torch.int32) % 100
+    slots = torch.arange(T, device="cuda", dtype=torch.int32)
+    k, v, k2, v2 = (empty_cache(pages_of(T, 16), hkv, 16, hd, torch.float32, "hnd", 0.0) for _ in range(4))
+    gain = 0.5 + torch.rand(hd, generator=gen(2), device="cuda")
+    opts = dict(n_heads=H, positions=pos, cos=cos, sin=sin, interleaved=il, q_norm=gain, k_norm=gain)
+    want = paged.append(x.clone(), k, v, slots, **opts)
+    y = x.clone()
+    paged.append(y, k2, v2, slots, out=y[:, : H * hd], **opts)
+    assert torch.equal(y[:, : H * hd], want) and torch.equal(y[:, H * hd:], x[:, H * hd:])
+    assert torch.equal(k, k2) and torch.equal(v, v2)
 
 
 def test_append_without_query_heads(paged):
