@@ -148,7 +148,7 @@ typedef struct sx_paged_attention_args {
   const int32_t* table; /* [n_req][table_stride] page ids */
   const int32_t* lens;  /* [n_req] */
   int32_t* status;
-  void* workspace; /* 16-byte aligned */
+  void* workspace; /* 16-byte aligned; null: no request is split, which short ones are not anyway */
   size_t workspace_bytes;
   int64_t q_stride, out_stride; /* elements, multiples of 16 bytes */
   int64_t table_stride;

@@ -1084,7 +1084,7 @@ template <class M>
 cudaError_t launch_m(AttnK a, long long bound, int sms, cudaStream_t st) {
   constexpr int TILE = 2 * M::TK * M::RB;
   const int partials = (M::NW - 1) * a.G * M::HD * 4;
-  a.direct = (long long)a.n * a.Hkv <= sms && bound <= (long long)kDirectTiles * M::NW * M::TK;
+  a.direct = !a.ws || ((long long)a.n * a.Hkv <= sms && bound <= (long long)kDirectTiles * M::NW * M::TK);
   const size_t smem = (size_t)M::NW * kStages * TILE + partials;
   // the joining kernel asks for the same split of L1 and shared memory, so that it can be resident
   // (and wait) while the first one runs

@@ -98,7 +98,7 @@ int paged_check(const sx_paged_attention_args& a, int sms) {
   if (rc) return rc;
   const sx_paged_cache& c = a.cache;
   if (a.n_req < 0) return refuse(SX_E_INVALID, "sx_paged_attention: negative n_req");
-  if (a.n_req > 0 && (!a.q || !a.out || !a.table || !a.lens || !a.workspace))
+  if (a.n_req > 0 && (!a.q || !a.out || !a.table || !a.lens))
     return refuse(SX_E_INVALID, "sx_paged_attention: null argument");
   if (a.q_dtype != SX_DTYPE_F32 && a.q_dtype != c.dtype)
     return refuse(SX_E_UNSUPPORTED, "sx_paged_attention: q is f32 or of the cache's type");
@@ -119,7 +119,7 @@ int paged_check(const sx_paged_attention_args& a, int sms) {
   if ((rc = check_row(a.out, a.out_stride, width, a.q_dtype, "sx_paged_attention: out"))) return rc;
   if (!aligned(a.workspace, 16)) return refuse(SX_E_INVALID, "sx_paged_attention: workspace must be 16-byte aligned");
   const size_t need = paged_attention_workspace(a.n_heads / c.n_kv_heads, c.head_dim, sms);
-  if (a.workspace_bytes < need)
+  if (a.workspace && a.workspace_bytes < need)
     return refuse(SX_E_RANGE, "sx_paged_attention: workspace holds " + std::to_string(a.workspace_bytes) + " bytes, " +
                                   std::to_string(need) + " needed");
   return SX_OK;

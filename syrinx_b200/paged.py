@@ -50,21 +50,20 @@ for _s, _c in ((_PLAN_ARGS, SxPagedPlanArgs), (_APPEND_ARGS, SxPagedAppendArgs),
     assert _s.size == C.sizeof(_c), "argument struct out of step with include/syrinx_paged.h"
 
 
-def _device(*tensors) -> int:
-    """The one CUDA device that the tensors (None: left out) are on."""
-    dev = tensors[0].get_device()
+def _on(dev: int, *tensors) -> None:
+    """Every tensor (None: left out) is on CUDA device `dev`."""
     if dev < 0:
         raise ValueError("the tensors must be on a CUDA device")
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError("the tensors must be on one device")
-    return dev
 
 
-def _ints(t: torch.Tensor, name: str, least: int) -> int:
-    if t.dtype is _I32 and t.is_contiguous() and t.numel() >= least:
+def _ints(dev: int, t: torch.Tensor, name: str, least: int) -> int:
+    """Address of a contiguous int32 tensor of at least `least` entries on device `dev`."""
+    if t.dtype is _I32 and t.get_device() == dev and t.is_contiguous() and t.numel() >= least:
         return t.data_ptr()
-    raise ValueError(f"{name}: a contiguous int32 tensor of at least {least} entries")
+    raise ValueError(f"{name}: a contiguous int32 tensor of at least {least} entries on the same CUDA device")
 
 
 def _row(t: torch.Tensor) -> int:
@@ -72,11 +71,15 @@ def _row(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.numel()
 
 
-def _table(t: torch.Tensor, n: int) -> int:
+def _table(dev: int, t: torch.Tensor, n: int) -> tuple:
+    """Address, elements from row to row and pages a row of a block table."""
     s = t.shape
-    if t.dtype is not _I32 or len(s) != 2 or s[0] < n or s[1] < 1 or t.stride(1) != 1:
-        raise ValueError("table: int32 [requests, pages] with contiguous rows")
-    return t.data_ptr()
+    if t.dtype is not _I32 or len(s) != 2 or s[0] < n or s[1] < 1 or t.get_device() != dev:
+        raise ValueError("table: int32 [requests, pages] on the same CUDA device")
+    row, step = t.stride()
+    if step != 1:
+        raise ValueError("table: a row's pages must be contiguous")
+    return t.data_ptr(), row if s[0] > 1 else s[1], s[1]
 
 
 def _cache(k: torch.Tensor, v: torch.Tensor, layout: str) -> tuple:
@@ -103,17 +106,19 @@ def plan(lens, delta, table, free_pages, n_free, *, page_size: int, slots=None, 
     lens_out = lens if lens_out is None else lens_out
     n_free_out = n_free if n_free_out is None else n_free_out
     if status is None:
-        status = torch.empty(4, dtype=torch.int32, device=lens.device)
-    dev = _device(lens, delta, table, free_pages, n_free, slots, tok_seq, tok_pos, starts, lens_out, n_free_out, status)
-    _need(most <= 0 or slots.dim() == 1, "slots: one dimension")
-    least = max(1, most)
+        status = torch.empty(4, dtype=_I32, device=lens.device)
+    dev, least = lens.get_device(), max(1, most)
+    if dev < 0:
+        raise ValueError("the tensors must be on a CUDA device")
+    address, stride, width = _table(dev, table, n)
     args = _PLAN_ARGS.pack(
-        _ints(lens, "lens", n), _ints(delta, "delta", n), _ints(n_free, "n_free", 1), _ints(lens_out, "lens_out", n),
-        _ints(n_free_out, "n_free_out", 1), _table(table, n), _ints(free_pages, "free_pages", 1),
-        _ints(slots, "slots", most) if most else 0, 0 if tok_seq is None else _ints(tok_seq, "tok_seq", least),
-        0 if tok_pos is None else _ints(tok_pos, "tok_pos", least),
-        0 if starts is None else _ints(starts, "starts", n + 1), _ints(status, "status", 4),
-        _row(table), table.shape[1], n, free_pages.shape[0], page_size, most, 0)
+        _ints(dev, lens, "lens", n), _ints(dev, delta, "delta", n), _ints(dev, n_free, "n_free", 1),
+        _ints(dev, lens_out, "lens_out", n), _ints(dev, n_free_out, "n_free_out", 1), address,
+        _ints(dev, free_pages, "free_pages", 1), _ints(dev, slots, "slots", most) if most else 0,
+        0 if tok_seq is None else _ints(dev, tok_seq, "tok_seq", least),
+        0 if tok_pos is None else _ints(dev, tok_pos, "tok_pos", least),
+        0 if starts is None else _ints(dev, starts, "starts", n + 1), _ints(dev, status, "status", 4),
+        stride, width, n, free_pages.shape[0], page_size, most, 0)
     _lib.check(_lib.lib().sx_paged_plan(args, dev, _stream(dev)))
     return status
 
@@ -133,7 +138,8 @@ def append(x, k, v, slots, *, n_heads: int, positions=None, cos=None, sin=None, 
     elif out.dim() != 2 or out.shape[0] < rows or out.shape[1] != n_heads * hd or out.dtype is not dtype or (
             out.stride(1) != 1 and out.shape[1] > 1):
         raise ValueError("out: [rows, n_heads * head_dim] of x's type")
-    dev = _device(x, k, v, slots, positions, cos, sin, q_norm, k_norm, out, status)
+    dev = x.get_device()
+    _on(dev, k, v, cos, sin, q_norm, k_norm, out)
     n_pos = 0
     if cos is not None or sin is not None:
         _need(cos is not None and sin is not None and cos.dtype is _F32 and sin.dtype is _F32
@@ -144,10 +150,10 @@ def append(x, k, v, slots, *, n_heads: int, positions=None, cos=None, sin=None, 
         _need(t is None or (t.dtype is _F32 and t.numel() == hd and t.is_contiguous()),
               "q_norm and k_norm: float32 [head_dim]")
     args = _APPEND_ARGS.pack(
-        *cache, x.data_ptr(), out.data_ptr() if n_heads else 0, _ints(slots, "slots", rows),
-        0 if positions is None else _ints(positions, "positions", rows), cos.data_ptr() if n_pos else 0,
+        *cache, x.data_ptr(), out.data_ptr() if n_heads else 0, _ints(dev, slots, "slots", rows),
+        0 if positions is None else _ints(dev, positions, "positions", rows), cos.data_ptr() if n_pos else 0,
         sin.data_ptr() if n_pos else 0, 0 if q_norm is None else q_norm.data_ptr(),
-        0 if k_norm is None else k_norm.data_ptr(), 0 if status is None else _ints(status, "status", 1),
+        0 if k_norm is None else k_norm.data_ptr(), 0 if status is None else _ints(dev, status, "status", 1),
         _row(x), _row(out), eps, _DTYPES[dtype], rows, n_heads, n_pos, int(interleaved))
     _lib.check(_lib.lib().sx_paged_append(args, dev, _stream(dev)))
     return out
@@ -168,7 +174,7 @@ def attend(q, k, v, table, lens, *, scale: float | None = None, layout: str = "h
     """Attention of one new token per request (sx_paged_attention): `q` [n, heads, head_dim] over the first
     `lens[i]` positions of the pages in `table[i]`; returns `out`, of q's shape and type. `scale` defaults to
     1 / sqrt(head_dim), `lse` [n, heads] float32 receives log sum exp. Without `workspace` (a tensor of
-    `workspace_bytes`) one is taken from torch's allocator for the call."""
+    `workspace_bytes`) one is taken from torch's allocator for the call, where the requests are split at all."""
     cache = _cache(k, v, layout)
     hkv, hd, dtype, shape = cache[8], cache[9], q.dtype, q.shape
     if len(shape) != 3 or shape[2] != hd or dtype not in _DTYPES:
@@ -180,22 +186,25 @@ def attend(q, k, v, table, lens, *, scale: float | None = None, layout: str = "h
         out = torch.empty((n, heads, hd), dtype=dtype, device=q.device)
     elif out.shape != shape or out.dtype is not dtype or out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd):
         raise ValueError("out: q's shape and type, a request's heads contiguous")
-    dev = _device(q, k, v, table, lens, out, lse, workspace, status)
+    dev = q.get_device()
+    _on(dev, k, v, out, lse, workspace)
     if n == 0:
         return out
-    size = _WORKSPACE.get((heads, hkv, hd, dev)) or workspace_bytes(heads, hkv, hd, dev)
-    if workspace is None:
-        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-    else:
+    address, stride, width = _table(dev, table, n)
+    pointer = size = 0  # few and short requests are not split, so they need no workspace
+    if workspace is not None:
         _need(workspace.is_contiguous(), "workspace must be contiguous")
-        size = workspace.numel() * workspace.element_size()
+        pointer, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif n * hkv > 64 or (max_len or width * cache[7]) > 256:
+        size = _WORKSPACE.get((heads, hkv, hd, dev)) or workspace_bytes(heads, hkv, hd, dev)
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+        pointer = workspace.data_ptr()
     if lse is not None and (lse.dtype is not _F32 or lse.numel() != n * heads or not lse.is_contiguous()):
         raise ValueError("lse: float32 [requests, heads]")
     args = _ATTEND_ARGS.pack(
-        *cache, q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), _table(table, n),
-        _ints(lens, "lens", n), 0 if status is None else _ints(status, "status", 1), workspace.data_ptr(), size,
-        _row(q), _row(out), _row(table), table.shape[1], n, heads, _DTYPES[dtype], max_len,
-        hd ** -0.5 if scale is None else scale)
+        *cache, q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), address,
+        _ints(dev, lens, "lens", n), 0 if status is None else _ints(dev, status, "status", 1), pointer, size,
+        _row(q), _row(out), stride, width, n, heads, _DTYPES[dtype], max_len, hd ** -0.5 if scale is None else scale)
     _lib.check(_lib.lib().sx_paged_attention(args, dev, _stream(dev)))
     return out
 

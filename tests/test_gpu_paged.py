@@ -361,6 +361,32 @@ def test_attend_reports_bad_pages_and_lengths(paged):
     assert (paged.attend(q, k, v, table, neg)[0] == 0).all()
 
 
+@pytest.mark.parametrize("qt,ct", TYPES)
+def test_attend_without_a_workspace(paged, qt, ct):
+    """The library call with a null workspace: nothing is split, whatever the lengths are."""
+    import ctypes as C
+
+    from syrinx_b200 import _lib
+    from syrinx_b200.configs import SxPagedAttentionArgs
+
+    lens = [5000, 0, 17, 900]
+    k, v, table = filled(lens, 2, 16, 64, DT[ct], "hnd", 31)
+    q = torch.randn((4, 8, 64), generator=gen(32), device="cuda").to(DT[qt])
+    out, d = torch.full_like(q, float("nan")), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    a = SxPagedAttentionArgs()
+    c = a.cache
+    c.k, c.v, c.page_stride, c.head_stride, c.token_stride = k.data_ptr(), v.data_ptr(), *k.stride()[:3]
+    kinds = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+    c.dtype, c.n_pages, c.page_size, c.n_kv_heads, c.head_dim = kinds[k.dtype], k.shape[0], 16, 2, 64
+    a.q, a.out, a.table, a.lens = q.data_ptr(), out.data_ptr(), table.data_ptr(), d.data_ptr()
+    a.q_stride = a.out_stride = 8 * 64
+    a.table_stride = a.table_width = table.shape[1]
+    a.n_req, a.n_heads, a.q_dtype, a.scale = 4, 8, kinds[q.dtype], 0.125
+    _lib.check(_lib.lib().sx_paged_attention(C.byref(a), 0, torch.cuda.current_stream().cuda_stream))
+    want, _, tol, _ = ref_attend(q, k, v, table, lens, 0.125, 16, "hnd")
+    assert ((out.double() - want).abs() <= tol).all()
+
+
 def test_attend_refusals(paged):
     import syrinx_b200 as sx
 

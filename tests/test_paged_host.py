@@ -87,7 +87,7 @@ APPEND = [
 ]
 ATTENTION = [
     (dict(q=None), INVALID), (dict(out=None), INVALID), (dict(table=None), INVALID), (dict(lens=None), INVALID),
-    (dict(workspace=None), INVALID), (dict(workspace_bytes=0), RANGE), (dict(workspace=P + 4), INVALID),
+    (dict(workspace_bytes=0), RANGE), (dict(workspace=P + 4), INVALID),
     (dict(n_req=-1), INVALID), (dict(q_dtype=1), UNSUPPORTED), (dict(n_heads=0), UNSUPPORTED),
     (dict(n_heads=33), UNSUPPORTED), (dict(n_heads=136), UNSUPPORTED), (dict(table_width=0), INVALID),
     (dict(table_stride=15), INVALID), (dict(max_len=-1), INVALID), (dict(q_stride=31 * 128), INVALID),
