@@ -47,6 +47,10 @@ struct Raw {
 #pragma unroll
     for (int i = 0; i < N; i++) w[i] = __ldcg(reinterpret_cast<const uint4*>(p) + i);
   }
+  __device__ __forceinline__ void store(void* p) const {
+#pragma unroll
+    for (int i = 0; i < N; i++) reinterpret_cast<uint4*>(p)[i] = w[i];
+  }
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < N; i++) w[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -76,15 +80,16 @@ struct Raw {
   }
 };
 
-// E values rounded once to T, as 16-byte words (8-byte where four 16-bit values are held).
+// E values rounded once to T, in as wide a word as they fill.
 template <typename T, int E>
-__device__ __forceinline__ void store_vec(T* p, const f32x2 (&v)[E / 2]) {
-  float x[E];
-#pragma unroll
-  for (int i = 0; i < E / 2; i++) unpack2(v[i], x[2 * i], x[2 * i + 1]);
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[E]) {
   if constexpr (sizeof(T) == 4) {
+    if constexpr (E == 2) {
+      *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < E; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      for (int i = 0; i < E; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+    }
   } else {
     uint32_t w[E / 2];
 #pragma unroll
@@ -97,11 +102,20 @@ __device__ __forceinline__ void store_vec(T* p, const f32x2 (&v)[E / 2]) {
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
       }
     }
-    if constexpr (E == 4)
+    if constexpr (E == 2)
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+    else if constexpr (E == 4)
       *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else
       *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
   }
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_vec(T* p, const f32x2 (&v)[E / 2]) {
+  float x[E];
+#pragma unroll
+  for (int i = 0; i < E / 2; i++) unpack2(v[i], x[2 * i], x[2 * i + 1]);
+  store_vec<T, E>(p, x);
 }
 
 // What the two kernels share: lanes e0 .. e0 + E - 1 of head h, of the row's H query, Hkv key
@@ -220,50 +234,157 @@ __global__ void __launch_bounds__(kAppendThreads) k_paged_append(const AppendK a
            a.q ? reinterpret_cast<XT*>(a.q + (size_t)row * a.q_stride) : nullptr, place_of(a, slot));
 }
 
-// Many rows: every warp walks an even run of units (kSteps steps of one row), copied ahead into
-// a ring of its own by cp.async together with the row's angles. A warp that loads a row's heads
-// into registers keeps too little in flight: 20 warps of 96 registers held 40 KB per SM and took
-// 97 us for 16384 rows of 48 bf16 heads of 128 (403 MB), where 24 warps with a ring take 80 us
-// (5.1 TB/s; without the norm it is the same: the mix of reads and writes bounds it).
+// Many rows: every warp walks an even run of units (up to kSteps steps of HW heads of one kind, query,
+// key or value, of one row), copied ahead into a ring of its own by cp.async together with the
+// row's angles. A warp that loads a row's heads into registers keeps too little in flight: 20
+// warps of 96 registers held 40 KB per SM and took 97 us for 16384 rows of 48 bf16 heads of 128
+// (403 MB); with the ring, whose instructions came to 160 per step, it took 80. So a unit is of one
+// kind and a head costs few instructions: gains, cosines and sines are multiplied together once
+// per unit, and a lane holds both elements of each pair it turns. That takes 69 us, 5.9 TB/s,
+// with two CTAs of rings of two units; more in flight is slower (three CTAs 79, three units 87:
+// reads and writes get in each other's way in HBM), less too (one CTA 96).
 constexpr int kSteps = 4;
-constexpr int kRing = 3;
+constexpr int kRing = 2;
 constexpr int kRingWarps = 8;
-// CTAs per SM: of f32 rows two keep as many bytes in flight as of 16-bit rows three (16384 rows of
-// 48 heads of 128: f32 158 us with three, 141 with two; bf16 80 and 87).
-template <typename XT>
-constexpr int ring_ctas() {
-  return sizeof(XT) == 4 ? 2 : 3;
-}
+constexpr int kRingCtas = 2;  // per SM
 
 template <int HD, typename XT, typename CT, bool IL>
 struct Unit {
   alignas(16) uint8_t x[kSteps * Head<HD, XT, CT, IL>::STEP];
   alignas(16) float angles[HD];  // cosines, sines
-  int slot, pad[3];
+};
+
+// A lane's E elements of a head as pairs (a, b) that are turned together: a' = r (a A + b B),
+// b' = r (b C + a D), r the head's norm factor. Interleaved pairs lie side by side, so the lane
+// holds E neighbours; half-head pairs lie HD / 2 apart, so it holds E / 2 of each half.
+template <int HD, typename XT, bool IL>
+struct Turn {
+  static constexpr int E = (sizeof(XT) == 4 && HD <= 128) ? 4 : 8;
+  static constexpr int N = E / 4;  // packed values of each side
+  f32x2 A[N], B[N], C[N], D[N];
+
+  // side 0 / 1 of pair i of lane t: its element of the head
+  static __device__ __forceinline__ int element(int t, int i, int side) {
+    return IL ? t * E + 2 * i + side : t * (E / 2) + i + side * (HD / 2);
+  }
+  // gain: this kind's gains; angles: cosines and sines, null for no rotation; t: lane of the head
+  __device__ __forceinline__ void set(const float* gain, const float* angles, int t) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      float k[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int p = 2 * i + j, at = t * (E / 2) + p;  // the pair, its angle
+        const float c = angles ? angles[at] : 1.f, s = angles ? angles[HD / 2 + at] : 0.f;
+        const float ga = gain[element(t, p, 0)], gb = gain[element(t, p, 1)];
+        k[j][0] = c * ga, k[j][1] = -s * gb, k[j][2] = c * gb, k[j][3] = s * ga;
+      }
+      A[i] = pack2(k[0][0], k[1][0]), B[i] = pack2(k[0][1], k[1][1]);
+      C[i] = pack2(k[0][2], k[1][2]), D[i] = pack2(k[0][3], k[1][3]);
+    }
+  }
+  // The lane's elements of the head at `p` in shared memory, as a and b sides.
+  static __device__ __forceinline__ void load(const uint8_t* p, int t, f32x2 (&a)[N], f32x2 (&b)[N]) {
+    constexpr int W = E * (int)sizeof(XT) / 4;  // words
+    uint32_t w[W];
+    if constexpr (IL) {
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        const uint4 r = *reinterpret_cast<const uint4*>(p + t * (W * 4) + i * 4);
+        w[i] = r.x, w[i + 1] = r.y, w[i + 2] = r.z, w[i + 3] = r.w;
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < W / 2; i += 2) {
+          const uint2 r = *reinterpret_cast<const uint2*>(p + t * (W * 2) + i * 4 + h * (HD / 2) * (int)sizeof(XT));
+          w[h * (W / 2) + i] = r.x, w[h * (W / 2) + i + 1] = r.y;
+        }
+    }
+    float x[E];
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+      if constexpr (sizeof(XT) == 4) {
+        x[i] = __uint_as_float(w[i]);
+      } else if constexpr (std::is_same<XT, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      } else {
+        x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      a[i] = IL ? pack2(x[4 * i], x[4 * i + 2]) : pack2(x[2 * i], x[2 * i + 1]);
+      b[i] = IL ? pack2(x[4 * i + 1], x[4 * i + 3]) : pack2(x[E / 2 + 2 * i], x[E / 2 + 2 * i + 1]);
+    }
+  }
+  static __device__ __forceinline__ float squares(const f32x2 (&a)[N], const f32x2 (&b)[N]) {
+    f32x2 q = mul2(a[0], a[0]);
+#pragma unroll
+    for (int i = 1; i < N; i++) q = fma2(a[i], a[i], q);
+#pragma unroll
+    for (int i = 0; i < N; i++) q = fma2(b[i], b[i], q);
+    float lo, hi;
+    unpack2(q, lo, hi);
+    return lo + hi;
+  }
+  // The turned elements to head `p` in type T.
+  template <typename T>
+  __device__ __forceinline__ void put(T* p, int t, const f32x2 (&a)[N], const f32x2 (&b)[N], float r, bool rotate) const {
+    const f32x2 by = pack2(r, r);
+    float y[E];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      f32x2 u = mul2(a[i], A[i]), v = mul2(b[i], C[i]);
+      if (rotate) u = fma2(b[i], B[i], u), v = fma2(a[i], D[i], v);
+      u = mul2(u, by), v = mul2(v, by);
+      if constexpr (IL) {
+        unpack2(u, y[4 * i], y[4 * i + 2]);
+        unpack2(v, y[4 * i + 1], y[4 * i + 3]);
+      } else {
+        unpack2(u, y[2 * i], y[2 * i + 1]);
+        unpack2(v, y[E / 2 + 2 * i], y[E / 2 + 2 * i + 1]);
+      }
+    }
+    if constexpr (IL) {
+      store_vec<T, E>(p + t * E, y);
+    } else {
+      float lo[E / 2], hi[E / 2];
+#pragma unroll
+      for (int i = 0; i < E / 2; i++) lo[i] = y[i], hi[i] = y[E / 2 + i];
+      store_vec<T, E / 2>(p + t * (E / 2), lo);
+      store_vec<T, E / 2>(p + t * (E / 2) + HD / 2, hi);
+    }
+  }
 };
 
 template <int HD, typename XT, typename CT, bool IL>
-__global__ void __launch_bounds__(kRingWarps * 32, ring_ctas<XT>()) k_paged_append_many(const AppendK a) {
+__global__ void __launch_bounds__(kRingWarps * 32, kRingCtas) k_paged_append_many(const AppendK a) {
   using P = Head<HD, XT, CT, IL>;
   using U = Unit<HD, XT, CT, IL>;
+  using T = Turn<HD, XT, IL>;
+  constexpr int E = P::E, HW = P::HW, LH = P::LH, HB = HD * (int)sizeof(XT);  // bytes of a head
   extern __shared__ __align__(16) uint8_t dyn[];
   __shared__ __align__(16) float gains[2][HD];
+  __shared__ __align__(16) float row_angles[kRingWarps][HD];  // of each warp's row
   pdl_launch_dependents();
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, e0 = lane % P::LH * P::E;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane / LH, t = lane % LH;
   for (int i = tid; i < HD; i += kRingWarps * 32) {
     gains[0][i] = a.qn ? a.qn[i] : 1.f;
     gains[1][i] = a.kn ? a.kn[i] : 1.f;
   }
   __syncthreads();
   U* ring = reinterpret_cast<U*>(dyn) + warp * kRing;
-  const int n_heads = a.H + 2 * a.Hkv, steps = (n_heads - a.first + P::HW - 1) / P::HW;
-  const int per_row = (steps + kSteps - 1) / kSteps;
+  // a row's units: nq of its query heads, nk of its key heads, nk of its value heads
+  constexpr int HU = kSteps * HW;  // heads per unit
+  const int nq = a.q ? (a.H + HU - 1) / HU : 0, nk = (a.Hkv + HU - 1) / HU, per_row = nq + 2 * nk;
   const long long units = (long long)a.rows * per_row, warps = (long long)gridDim.x * kRingWarps;
   const long long w = (long long)blockIdx.x * kRingWarps + warp;
   const long long u0 = units / warps * w + units % warps * w / warps;
   const long long u1 = units / warps * (w + 1) + units % warps * (w + 1) / warps;
-  const int row_bytes = n_heads * HD * (int)sizeof(XT);
 
   // the copying side: slots and positions of 32 rows, one per lane
   int row_p = (int)(u0 / per_row), unit_p = (int)(u0 % per_row), cached = -1, slots = 0, poss = 0;
@@ -281,18 +402,22 @@ __global__ void __launch_bounds__(kRingWarps * 32, ring_ctas<XT>()) k_paged_appe
           if (a.status) *a.status = SX_E_RANGE;
         }
       }
-      const int slot = __shfl_sync(0xffffffffu, slots, row_p - cached), pos = __shfl_sync(0xffffffffu, poss, row_p - cached);
-      U& to = ring[at];
-      if (lane == 0) to.slot = slot;
-      if (slot != -1) {
-        const int off = a.first * HD * (int)sizeof(XT) + unit_p * kSteps * P::STEP;
-        const uint8_t* src = a.x + (size_t)row_p * a.x_stride + off;
+      if (__shfl_sync(0xffffffffu, slots, row_p - cached) != -1) {
+        U& to = ring[at];
+        const int part = unit_p < nq ? 0 : unit_p < nq + nk ? 1 : 2;
+        const int h = (part == 0 ? unit_p : part == 1 ? unit_p - nq : unit_p - nq - nk) * HU;  // first head, of its kind
+        const int bytes = min(HU, (part == 0 ? a.H : a.Hkv) - h) * HB;
+        const uint8_t* src = a.x + (size_t)row_p * a.x_stride + (uint32_t)(h + (part == 0 ? 0 : part == 1 ? a.H : a.H + a.Hkv)) * HB +
+                             lane * 16;
+        const uint32_t dst = smem_addr(to.x) + lane * 16;
+        if (bytes == HU * HB) {
 #pragma unroll
-        for (int x = 0; x < kSteps * P::STEP / 512; x++) {
-          const int b = x * 512 + lane * 16;
-          cp_async16(smem_addr(to.x + b), off + b < row_bytes ? src + b : a.x, off + b < row_bytes ? 16 : 0);
+          for (int b = 0; b < HU * HB; b += 512) cp_async16(dst + b, src + b, 16);
+        } else {
+          for (int b = lane * 16; b < bytes; b += 512) cp_async16(dst + b - lane * 16, src + b - lane * 16, 16);
         }
         if (a.cosv && (fresh || unit_p == 0)) {
+          const int pos = __shfl_sync(0xffffffffu, poss, row_p - cached);
 #pragma unroll
           for (int b = lane * 16; b < HD * 4; b += 512)
             cp_async16(smem_addr(to.angles) + b,
@@ -306,53 +431,88 @@ __global__ void __launch_bounds__(kRingWarps * 32, ring_ctas<XT>()) k_paged_appe
     cp_commit();
   };
   int into = 0, from = 0;
-#pragma unroll
+#pragma unroll 1
   for (int x = 0; x < kRing - 1; x++) {
     copy_next(into);
-    into = (into + 1) % kRing;
+    into = into + 1 == kRing ? 0 : into + 1;
   }
-  int row = (int)(u0 / per_row), unit = (int)(u0 % per_row);
+  int row = (int)(u0 / per_row), unit = (int)(u0 % per_row), held = -1, slot_of = 0;
   bool first = true;
-  P head;
+  T turn;
+  float* angles = row_angles[warp];
   for (long long todo = u1 - u0; todo > 0; todo--) {
     copy_next(into);
-    into = (into + 1) % kRing;
+    into = into + 1 == kRing ? 0 : into + 1;
     cp_wait<kRing - 1>();
     __syncwarp();
     const U& u = ring[from];
-    from = (from + 1) % kRing;
-    const int slot = u.slot;
+    from = from + 1 == kRing ? 0 : from + 1;
+    if (held < 0 || row >= held + 32) {  // as the copying side, which is ahead
+      held = row;
+      slot_of = row + lane < a.rows ? ld_cg(a.slots + row + lane) : -1;
+      const int pos = row + lane < a.rows && a.cosv ? ld_cg(a.pos + row + lane) : 0;
+      if (slot_of != -1 && refuses(a, slot_of, pos)) slot_of = -1;
+    }
+    const int slot = __shfl_sync(0xffffffffu, slot_of, row - held);
     if (slot != -1) {
-      if (a.cosv && (first || unit == 0)) head.angles(u.angles, u.angles + HD / 2, e0);
-      float ss[kSteps];
-      if (a.qn || a.kn) {
-        // the sums of all steps first: their shuffles do not wait for one another
+      const int part = unit < nq ? 0 : unit < nq + nk ? 1 : 2;
+      const int h0 = (part == 0 ? unit : part == 1 ? unit - nq : unit - nq - nk) * HU;
+      const int left = (part == 0 ? a.H : a.Hkv) - h0 - sub;  // heads of this lane's: left > x HW
+      if (a.cosv && (first || unit == 0)) {
+        for (int i = lane; i < HD / 4; i += 32)
+          reinterpret_cast<float4*>(angles)[i] = reinterpret_cast<const float4*>(u.angles)[i];
+        __syncwarp();
+      }
+      CT* kv = reinterpret_cast<CT*>(part == 1 ? a.k : a.v) + place_of(a, slot) + (size_t)(h0 + sub) * a.head_stride;
+      if (part == 2) {
 #pragma unroll
         for (int x = 0; x < kSteps; x++) {
-          Raw<XT, P::E> raw;
-          raw.load_shared(u.x + x * P::STEP + lane * (P::E * (int)sizeof(XT)));
-          f32x2 v[P::E / 2];
-          raw.values(v);
-          ss[x] = P::squares(v);
+          if (left <= x * HW) break;
+          Raw<XT, E> raw;
+          raw.load_shared(u.x + (x * 32 + lane) * (E * (int)sizeof(XT)));
+          CT* to = kv + (size_t)(x * HW) * a.head_stride + t * E;
+          if constexpr (std::is_same<XT, CT>::value) {
+            raw.store(to);
+          } else {
+            f32x2 v[E / 2];
+            raw.values(v);
+            store_vec<CT, E>(to, v);
+          }
         }
+      } else {
+        const float* gain = part == 0 ? a.qn : a.kn;
+        turn.set(gains[part], a.cosv ? angles : nullptr, t);
+        const uint8_t* mine = u.x + sub * HB;
+        float r[kSteps];
+        if (gain) {
+          // the sums of all steps first: their shuffles do not wait for one another
 #pragma unroll
-        for (int o = P::LH / 2; o > 0; o >>= 1)
+          for (int x = 0; x < kSteps; x++) {
+            f32x2 va[T::N], vb[T::N];
+            T::load(mine + x * HW * HB, t, va, vb);
+            r[x] = T::squares(va, vb);
+          }
 #pragma unroll
-          for (int x = 0; x < kSteps; x++) ss[x] += __shfl_xor_sync(0xffffffffu, ss[x], o);
-      }
-      XT* q = a.q ? reinterpret_cast<XT*>(a.q + (size_t)row * a.q_stride) : nullptr;
-      const size_t cache = place_of(a, slot);
+          for (int o = LH / 2; o > 0; o >>= 1)
 #pragma unroll
-      for (int x = 0; x < kSteps; x++) {
-        const int h0 = a.first + (unit * kSteps + x) * P::HW;
-        if (h0 >= n_heads) break;
-        const int h = h0 + lane / P::LH;
-        Raw<XT, P::E> raw;
-        raw.load_shared(u.x + x * P::STEP + lane * (P::E * (int)sizeof(XT)));
-        f32x2 v[P::E / 2];
-        raw.values(v);
-        const float* gain = h < a.H ? (a.qn ? gains[0] : nullptr) : h < a.H + a.Hkv && a.kn ? gains[1] : nullptr;
-        head.put(a, v, ss[x] * (1.f / HD), gain, h, e0, q, cache);
+            for (int x = 0; x < kSteps; x++) r[x] += __shfl_xor_sync(0xffffffffu, r[x], o);
+#pragma unroll
+          for (int x = 0; x < kSteps; x++) r[x] = rsqrtf(fmaf(r[x], 1.f / HD, a.eps));
+        } else {
+#pragma unroll
+          for (int x = 0; x < kSteps; x++) r[x] = 1.f;
+        }
+        XT* q = reinterpret_cast<XT*>(a.q + (size_t)row * a.q_stride) + (uint32_t)(h0 + sub) * HD;
+#pragma unroll
+        for (int x = 0; x < kSteps; x++) {
+          if (left <= x * HW) break;
+          f32x2 va[T::N], vb[T::N];
+          T::load(mine + x * HW * HB, t, va, vb);
+          if (part == 0)
+            turn.template put<XT>(q + x * HW * HD, t, va, vb, r[x], a.cosv);
+          else
+            turn.template put<CT>(kv + (size_t)(x * HW) * a.head_stride, t, va, vb, r[x], a.cosv);
+        }
       }
     }
     first = false;
@@ -368,10 +528,10 @@ cudaError_t launch_t(AppendK a, int sms, cudaStream_t st) {
   a.first = a.q ? 0 : a.H;
   const int steps = (a.H - a.first + 2 * a.Hkv + P::HW - 1) / P::HW;
   cudaLaunchAttribute attr[1];
-  // A warp per step up to about two waves of them; beyond, its start-up is paid too often (48 bf16
-  // heads of 128: 300 rows 4.1 us against 5.6 with the ring, 600 6.2 / 6.8, 1200 10.8 / 10.0,
-  // 5000 40 / 30).
-  if ((long long)a.rows * steps <= 96ll * sms && steps <= 65535) {
+  // A warp per step up to about three waves of them (48 bf16 heads of 128: 300 rows 4.1 us against
+  // 5.6 with the ring, 600 6.2 / 5.9, 1200 10.8 / 8.9, 5000 40 / 25), and for narrow rows, which are
+  // only a few units (14 + 2 x 2 bf16 heads of 64: 5000 rows 8.6 / 11.6, 16384 27.4 / 30.2).
+  if (((long long)a.rows * steps <= 144ll * sms || steps <= 8) && steps <= 65535) {
     constexpr int W = kAppendThreads / 32;
     cudaLaunchConfig_t cfg = launch_cfg(dim3((a.rows + W - 1) / W, steps), dim3(kAppendThreads), 0, st, attr);
     return cudaLaunchKernelEx(&cfg, k_paged_append<HD, XT, CT, IL>, a);
@@ -387,9 +547,10 @@ cudaError_t launch_t(AppendK a, int sms, cudaStream_t st) {
       return e;
     if (device < 64) ready.fetch_or(1ull << device, std::memory_order_release);
   }
-  // beside the ring a CTA holds its gains and 1 KB of the system's
-  const int per_sm = std::max(1, std::min(ring_ctas<XT>(), (226 * 1024) / (smem + 3072)));
-  const long long units = (long long)a.rows * ((steps + kSteps - 1) / kSteps);
+  // beside the ring a CTA holds gains, its rows' angles and 1 KB of the system's
+  const int per_sm = std::max(1, std::min(kRingCtas, (226 * 1024) / (smem + 1024 + (2 + kRingWarps) * HD * 4)));
+  constexpr int HU = kSteps * P::HW;
+  const long long units = (long long)a.rows * ((a.q ? (a.H + HU - 1) / HU : 0) + 2 * ((a.Hkv + HU - 1) / HU));
   const int grid = (int)std::min<long long>((long long)per_sm * sms, (units + kRingWarps - 1) / kRingWarps);
   cudaLaunchConfig_t cfg = launch_cfg(dim3(grid), dim3(kRingWarps * 32), smem, st, attr);
   return cudaLaunchKernelEx(&cfg, k_paged_append_many<HD, XT, CT, IL>, a);
