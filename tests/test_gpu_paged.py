@@ -534,6 +534,61 @@ def test_append_many_rows(paged, xt, ct):
     assert_appends(paged, 3001, 5, 16, 8, 64, 32, xt, ct, "nhd", (1, 1), 1, False, 3, strided=True)
 
 
+@pytest.mark.parametrize("xt,ct", TYPES)
+@pytest.mark.parametrize("H,hkv,hd", [(70, 5, 32), (40, 3, 64), (21, 5, 128), (9, 2, 256)])
+@pytest.mark.parametrize("norm,rot,il", [((1, 1), 1, 1), ((1, 1), 1, 0), ((0, 1), 0, 0), ((1, 0), 1, 0), ((0, 0), 0, 1)])
+def test_append_many_wide_rows(paged, xt, ct, H, hkv, hd, norm, rot, il):
+    """Heads that do not fill the last step or unit of their kind, over many rows."""
+    assert_appends(paged, 3000, 2, H, hkv, hd, 16, xt, ct, "nhd" if il else "hnd", norm, rot, bool(il), 5, strided=True)
+
+
+@pytest.mark.parametrize("xt,ct", [("f32", "bf16"), ("bf16", "bf16")])
+def test_append_many_rows_with_bad_ones(paged, xt, ct):
+    """Rows without a slot, and with a slot or a position that is none."""
+    H, hkv, hd, T = 6, 20, 128, 2000
+    x = torch.randn((T, (H + 2 * hkv) * hd), generator=gen(3), device="cuda").to(DT[xt])
+    k, v = (empty_cache(pages_of(T, 16), hkv, 16, hd, DT[ct], "nhd", 7.0) for _ in range(2))
+    slots = torch.arange(T, device="cuda", dtype=torch.int32)
+    pos = torch.arange(T, device="cuda", dtype=torch.int32) % 50
+    slots[5::97], slots[6::97], pos[7::97] = -1, pages_of(T, 16) * 16, 50
+    cos, sin = rope(50, hd)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    paged.append(x, k, v, slots, n_heads=H, positions=pos, cos=cos, sin=sin, layout="nhd", status=status)
+    assert int(status) == -7
+    good = (slots >= 0) & (slots < pages_of(T, 16) * 16) & (pos < 50)
+    y, tol = ref_append(x[good], H, hkv, hd, pos[good], cos, sin, True, None, None, 1e-6)
+    flat = k.view(-1, hkv, hd)[:T]
+    assert ((flat[good].double() - y[:, H:H + hkv]).abs() <= tol[:, H:H + hkv] + rounding(DT[ct], y[:, H:H + hkv])).all()
+    assert (flat[~good] == 7).all() and (v.view(-1, hkv, hd)[:T][~good] == 7).all()
+
+
+@pytest.mark.parametrize("T", [70, 3000])
+def test_append_drops_queries(paged, T):
+    """The library call with a null q_out: keys and values as with one."""
+    import ctypes as C
+
+    from syrinx_b200 import _lib
+    from syrinx_b200.configs import SxPagedAppendArgs
+
+    H, hkv, hd = 6, 12, 128
+    x = torch.randn((T, (H + 2 * hkv) * hd), generator=gen(3), device="cuda")
+    slots = torch.randperm(pages_of(T, 64) * 64, generator=gen(4), device="cuda")[:T].to(torch.int32)
+    pos = torch.arange(T, device="cuda", dtype=torch.int32) % 50
+    cos, sin = rope(50, hd)
+    gain = 0.5 + torch.rand(hd, generator=gen(2), device="cuda")
+    k, v, k2, v2 = (empty_cache(pages_of(T, 64), hkv, 64, hd, torch.float32, "hnd", 7.0) for _ in range(4))
+    paged.append(x, k, v, slots, n_heads=H, positions=pos, cos=cos, sin=sin, k_norm=gain)
+    a = SxPagedAppendArgs()
+    c = a.cache
+    c.k, c.v, c.page_stride, c.head_stride, c.token_stride = k2.data_ptr(), v2.data_ptr(), *k2.stride()[:3]
+    c.dtype, c.n_pages, c.page_size, c.n_kv_heads, c.head_dim = 0, k2.shape[0], 64, hkv, hd
+    a.x, a.slots, a.positions, a.cos, a.sin = (t.data_ptr() for t in (x, slots, pos, cos, sin))
+    a.k_norm, a.x_stride, a.eps = gain.data_ptr(), x.shape[1], 1e-6
+    a.x_dtype, a.n_rows, a.n_heads, a.n_positions, a.interleaved = 0, T, H, 50, 1
+    _lib.check(_lib.lib().sx_paged_append(C.byref(a), 0, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(k, k2) and torch.equal(v, v2)
+
+
 @pytest.mark.parametrize("T", [3, 4000])
 @pytest.mark.parametrize("il", [True, False])
 def test_append_queries_in_place(paged, T, il):
@@ -555,6 +610,7 @@ def test_append_queries_in_place(paged, T, il):
 
 def test_append_without_query_heads(paged):
     assert_appends(paged, 9, 0, 0, 2, 128, 16, "f32", "bf16", "hnd", (0, 1), 1, True, 4)
+    assert_appends(paged, 2500, 1, 0, 12, 128, 16, "f32", "bf16", "hnd", (0, 1), 1, True, 4)
 
 
 def test_append_reports_bad_slots_and_positions(paged):
