@@ -80,7 +80,7 @@ __device__ __forceinline__ void put4(float* p, float x, float y, float z, float 
 }
 template <typename T>
 __device__ __forceinline__ void put4(T* p, float x, float y, float z, float w) {
-  T v[4];
+  alignas(8) T v[4];
   put(v, x), put(v + 1, y), put(v + 2, z), put(v + 3, w);
   *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
 }
