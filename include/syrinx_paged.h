@@ -154,7 +154,7 @@ typedef struct sx_paged_attention_args {
   int64_t table_stride;
   int32_t table_width;
   int32_t n_req;   /* 0: nothing is done; n_req x kv heads x tiles of a row below 2^32 */
-  int32_t n_heads; /* n_kv_heads x 1 .. 16 (1 .. 8 at head_dim 256) */
+  int32_t n_heads; /* a multiple of n_kv_heads */
   int32_t q_dtype; /* SX_DTYPE_F32, or the cache's type */
   int32_t max_len; /* what no length exceeds, as far as the host knows (0: table_width pages);
                       it chooses the launch and never the result's meaning */

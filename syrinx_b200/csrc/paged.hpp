@@ -20,6 +20,8 @@ cudaError_t launch_paged_attention(const sx_paged_attention_args& a, int sms, cu
 constexpr int kPagedSegTiles = 2;
 // Most tiles and (request, kv head) pairs that the call's table can hold: they are counted in 32 bits.
 int64_t paged_attention_cost(const sx_paged_attention_args& a);
+// Query heads of a kv head (of G) that are run together.
+int paged_attention_group(int G, int hd, bool f32);
 size_t paged_attention_workspace(int G, int hd, int sms);
 
 // ---- pooled sessions (pool.cu) --------------------------------------------------------------

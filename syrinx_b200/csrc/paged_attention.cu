@@ -54,10 +54,20 @@ struct AttnK {
   long long q_stride, out_stride;                    // elements
   long long page_stride, head_stride, token_stride;  // bytes
   long long table_stride;
-  int n, Hkv, G, H, page_shift, width, n_pages;
+  // a kv head's Gall query heads are run as `share` groups of up to G; Hkv counts the groups of all
+  int n, Hkv, G, H, page_shift, width, n_pages, Gall, share;
   int direct;  // 1: CTA c is (request c / Hkv, kv head c % Hkv); nothing is split over CTAs
   float scale;
 };
+
+// Of group h: its kv head, its first query head, and how many it has.
+__device__ __forceinline__ int kv_head(const AttnK& a, int h) { return a.share == 1 ? h : h / a.share; }
+__device__ __forceinline__ int first_head(const AttnK& a, int h) {
+  return a.share == 1 ? h * a.G : h / a.share * a.Gall + h % a.share * a.G;
+}
+__device__ __forceinline__ int group_heads(const AttnK& a, int h) {
+  return a.share == 1 ? a.G : min(a.G, a.Gall - h % a.share * a.G);
+}
 
 // Workspace: per CTA a record of the partial that begins in it, then two partials per CTA
 // (the one its share begins inside of, the one it ends inside of).
@@ -219,12 +229,13 @@ struct Mma {
 
   __device__ __forceinline__ void start(const AttnK& a, int i, int h, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    const QT* qp = reinterpret_cast<const QT*>(a.q) + (size_t)i * a.q_stride + (size_t)h * a.G * HD;
+    const QT* qp = reinterpret_cast<const QT*>(a.q) + (size_t)i * a.q_stride + (size_t)first_head(a, h) * HD;
+    const int heads = group_heads(a, h);
     const float base = a.scale * kLog2e;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const int head = nt * 8 + g;
-      const bool on = head < a.G;
+      const bool on = head < heads;
       float up = 1.f, down = 1.f;  // powers of two
       if constexpr (kQ32) {
         float2 x[KS][2];
@@ -458,13 +469,14 @@ struct Fma {
 
   __device__ __forceinline__ void start(const AttnK& a, int i, int h, int lane) {
     const int hs = lane % LPK;
-    const float* qp = reinterpret_cast<const float*>(a.q) + (size_t)i * a.q_stride + (size_t)h * a.G * HD;
+    const float* qp = reinterpret_cast<const float*>(a.q) + (size_t)i * a.q_stride + (size_t)first_head(a, h) * HD;
+    const int heads = group_heads(a, h);
     sl2 = a.scale * kLog2e;
 #pragma unroll
     for (int g = 0; g < GM; g++) {
 #pragma unroll
       for (int j = 0; j < E / 4; j++) {
-        const float4 x = g < a.G ? __ldcg(reinterpret_cast<const float4*>(qp + (size_t)g * HD) + hs + LPK * j)
+        const float4 x = g < heads ? __ldcg(reinterpret_cast<const float4*>(qp + (size_t)g * HD) + hs + LPK * j)
                                  : make_float4(0.f, 0.f, 0.f, 0.f);
         q[g][2 * j] = pack2(x.x, x.y);
         q[g][2 * j + 1] = pack2(x.z, x.w);
@@ -855,7 +867,7 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
       const int left = pp.len - key0;
       if (page_mask >= TK - 1) {  // the tile lies in one page
         const int page = __shfl_sync(0xffffffffu, pages, p0 - page_base);
-        size_t off = (size_t)(page < 0 ? 0 : page) * a.page_stride + (size_t)pp.h * a.head_stride +
+        size_t off = (size_t)(page < 0 ? 0 : page) * a.page_stride + (size_t)kv_head(a, pp.h) * a.head_stride +
                      (size_t)((key0 & page_mask) + lane / CPR) * a.token_stride + lane % CPR * 16;
         const int rows = page < 0 ? 0 : left;
         const size_t down = (CPR <= 32 ? 32 / CPR : 1) * a.token_stride;
@@ -877,7 +889,7 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
           const int key = key0 + r;
           const int page = __shfl_sync(0xffffffffu, pages, (key >> a.page_shift) - page_base);
           const int bytes = r < left && page >= 0 ? 16 : 0;
-          const size_t at = bytes ? (size_t)page * a.page_stride + (size_t)pp.h * a.head_stride +
+          const size_t at = bytes ? (size_t)page * a.page_stride + (size_t)kv_head(a, pp.h) * a.head_stride +
                                         (size_t)(key & page_mask) * a.token_stride + c * 16
                                   : 0;
           cp_async16(dst + M::at(r, c), a.k + at, bytes);
@@ -918,13 +930,14 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
     const bool done = !before_last(pc);
     if (rest == 0 || done) {
       if (rest == 0 && began) {
-        QT* out = reinterpret_cast<QT*>(a.out) + (size_t)i * a.out_stride + (size_t)h * a.G * HD;
+        const int head0 = first_head(a, h);
+        QT* out = reinterpret_cast<QT*>(a.out) + (size_t)i * a.out_stride + (size_t)head0 * HD;
         mine.finish(
-            a.G, lane, [&](float sum) { return sum == 0.f ? 0.f : __fdiv_rn(1.f, sum); },
+            group_heads(a, h), lane, [&](float sum) { return sum == 0.f ? 0.f : __fdiv_rn(1.f, sum); },
             [&](int head, int d, float v) { put(out + head * HD + d, v); },
             [&](int head, float top, float sum) {
               if (a.lse)
-                a.lse[(size_t)i * a.H + (size_t)h * a.G + head] =
+                a.lse[(size_t)i * a.H + head0 + head] =
                     sum == 0.f ? -INFINITY : kLn2 * (finite_or_zero(top) + log2f(sum) - M::kLift);
             });
       } else {
@@ -936,7 +949,7 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
                                   : first_o + (size_t)(warp - 1) * a.G * HD;
         float2* ml = out_of_cta ? ws_ml + (size_t)2 * cta * a.G : sm.ml[slot];
         mine.finish(
-            a.G, lane, [](float) { return 1.f; }, [&](int head, int d, float v) { dst[head * HD + d] = v; },
+            group_heads(a, h), lane, [](float) { return 1.f; }, [&](int head, int d, float v) { dst[head * HD + d] = v; },
             [&](int head, float top, float sum) { ml[head] = make_float2(top, sum); });
         if (lane == 0 && !out_of_cta)
           sm.piece[slot] = make_int4(i, h, kValid | (began ? kBegins : 0) | (rest == 0 ? kEnds : 0), rest);
@@ -971,7 +984,8 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
         *reinterpret_cast<int4*>(joint + cta) = make_int4(i, h, 1 + (int)((tail_piece.w + share - 1) / share), 0);
     }
     if (team != k % teams) continue;
-    for (int e = tid - team * team_size; e < a.G * (HD / 4); e += team_size) {
+    const int head0 = first_head(a, h), heads = group_heads(a, h);
+    for (int e = tid - team * team_size; e < heads * (HD / 4); e += team_size) {
       const int head = e / (HD / 4);
       float top = -INFINITY;
 #pragma unroll 1
@@ -992,10 +1006,10 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
       if (begins && ends) {
         const float inv = sum == 0.f ? 0.f : __fdiv_rn(1.f, sum);
         if (sum == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
-        put4(reinterpret_cast<QT*>(a.out) + (size_t)i * a.out_stride + (size_t)h * a.G * HD + 4 * e, v.x * inv, v.y * inv,
+        put4(reinterpret_cast<QT*>(a.out) + (size_t)i * a.out_stride + (size_t)head0 * HD + 4 * e, v.x * inv, v.y * inv,
              v.z * inv, v.w * inv);
         if (a.lse && e % (HD / 4) == 0)
-          a.lse[(size_t)i * a.H + (size_t)h * a.G + head] =
+          a.lse[(size_t)i * a.H + head0 + head] =
               sum == 0.f ? -INFINITY : kLn2 * (ref + log2f(sum) - M::kLift);
       } else {
         reinterpret_cast<float4*>(ws_o)[(size_t)slot * a.G * (HD / 4) + e] = v;
@@ -1035,7 +1049,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const AttnK a, int 
   }
   float top = __ldcg(ml + slot(min(tid, most - 1))).x;
   const int pieces = joint.z;
-  if (pieces == 0) return;
+  if (pieces == 0 || head >= group_heads(a, joint.y)) return;
   if (tid >= pieces) top = -INFINITY;
   for (int y = tid + kJoinThreads; y < pieces; y += kJoinThreads) top = fmaxf(top, __ldcg(ml + slot(y)).x);
   top = warp_max(top);
@@ -1059,7 +1073,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const AttnK a, int 
   acc[tid] = v;
   if (c == 0) sums[group] = sum;
   __syncthreads();
-  const size_t row = (size_t)joint.y * a.G + head;
+  const size_t row = (size_t)first_head(a, joint.y) + head;
   float total = 0.f;
 #pragma unroll
   for (int g = 0; g < GROUPS; g++) total += sums[g];
@@ -1114,13 +1128,12 @@ cudaError_t launch_hd(const AttnK& a, long long bound, int sms, cudaStream_t st)
   if constexpr (sizeof(CT) == 4) {
     if (a.G <= 2) return launch_m<Fma<HD, 2>>(a, bound, sms, st);
     if (a.G <= 4) return launch_m<Fma<HD, 4>>(a, bound, sms, st);
-    if (a.G <= 8) return launch_m<Fma<HD, 8>>(a, bound, sms, st);
-    if constexpr (HD < 256) return launch_m<Fma<HD, 16>>(a, bound, sms, st);
+    return launch_m<Fma<HD, 8>>(a, bound, sms, st);
   } else {
     if (a.G <= 8) return launch_m<Mma<HD, QT, CT, 8>>(a, bound, sms, st);
     if constexpr (HD < 256) return launch_m<Mma<HD, QT, CT, 16>>(a, bound, sms, st);
   }
-  return cudaErrorInvalidValue;
+  return cudaErrorInvalidValue;  // not reached: group_limit
 }
 
 template <typename QT, typename CT>
@@ -1135,7 +1148,15 @@ cudaError_t launch_t(const AttnK& a, int hd, long long bound, int sms, cudaStrea
 
 }  // namespace
 
-size_t paged_attention_workspace(int G, int hd, int sms) { return ws_bytes(sms, G, hd); }
+// Query heads that one pass over a kv head's tiles serves; more are run as groups, which read the
+// tiles again (from L2, as neighbours in the line). f32 pages: 16 heads at once kept too little of
+// their work in registers, 1.4 TB/s where two groups of 8 reach 2.4.
+int paged_attention_group(int G, int hd, bool f32) {
+  const int most = f32 || hd == 256 ? 8 : 16, share = (G + most - 1) / most;
+  return (G + share - 1) / share;
+}
+
+size_t paged_attention_workspace(int G, int hd, int sms) { return ws_bytes(sms, paged_attention_group(G, hd, false), hd); }
 
 cudaError_t launch_paged_attention(const sx_paged_attention_args& a, int sms, cudaStream_t st) {
   AttnK k;
@@ -1156,9 +1177,11 @@ cudaError_t launch_paged_attention(const sx_paged_attention_args& a, int sms, cu
   k.token_stride = a.cache.token_stride * ce;
   k.table_stride = a.table_stride;
   k.n = a.n_req;
-  k.Hkv = a.cache.n_kv_heads;
   k.H = a.n_heads;
-  k.G = a.n_heads / a.cache.n_kv_heads;
+  k.Gall = a.n_heads / a.cache.n_kv_heads;
+  k.G = paged_attention_group(k.Gall, a.cache.head_dim, a.cache.dtype == SX_DTYPE_F32);
+  k.share = (k.Gall + k.G - 1) / k.G;
+  k.Hkv = a.cache.n_kv_heads * k.share;
   k.page_shift = __builtin_ctz((unsigned)a.cache.page_size);
   k.width = a.table_width;
   k.n_pages = a.cache.n_pages;

@@ -102,16 +102,15 @@ int paged_check(const sx_paged_attention_args& a, int sms) {
     return refuse(SX_E_INVALID, "sx_paged_attention: null argument");
   if (a.q_dtype != SX_DTYPE_F32 && a.q_dtype != c.dtype)
     return refuse(SX_E_UNSUPPORTED, "sx_paged_attention: q is f32 or of the cache's type");
-  const int most = c.head_dim == 256 ? 8 : 16;
-  if (a.n_heads < 1 || a.n_heads % c.n_kv_heads || a.n_heads / c.n_kv_heads > most)
-    return refuse(SX_E_UNSUPPORTED, "sx_paged_attention: n_heads must be a multiple (<= " + std::to_string(most) +
-                                        "x at this head_dim) of n_kv_heads");
+  if (a.n_heads < 1 || a.n_heads % c.n_kv_heads)
+    return refuse(SX_E_UNSUPPORTED, "sx_paged_attention: n_heads must be a multiple of n_kv_heads");
+  if (a.n_heads > (1 << 16)) return refuse(SX_E_RANGE, "sx_paged_attention: too many heads");
   if (a.table_width < 1 || a.table_stride < a.table_width || a.max_len < 0)
     return refuse(SX_E_INVALID, "sx_paged_attention: bad table width or stride, or negative max_len");
   if ((int64_t)a.table_width * c.page_size > INT32_MAX)
     return refuse(SX_E_RANGE, "sx_paged_attention: a row's positions must be below 2^31");
-  if ((int64_t)a.n_req * c.n_kv_heads > INT32_MAX)
-    return refuse(SX_E_RANGE, "sx_paged_attention: n_req * n_kv_heads must be below 2^31");
+  if ((int64_t)a.n_req * a.n_heads > INT32_MAX)
+    return refuse(SX_E_RANGE, "sx_paged_attention: n_req * n_heads must be below 2^31");
   if (paged_attention_cost(a) > UINT32_MAX)
     return refuse(SX_E_RANGE, "sx_paged_attention: requests x kv heads x a row's positions is too large for one call");
   const int64_t width = (int64_t)a.n_heads * c.head_dim;
@@ -129,7 +128,8 @@ int64_t paged_attention_cost(const sx_paged_attention_args& a) {
   const int hd = a.cache.head_dim;
   const int keys = a.cache.dtype == SX_DTYPE_F32 ? 1024 / hd : hd == 32 ? 64 : hd == 64 ? 32 : 16;
   const int64_t tiles = ((int64_t)a.table_width * a.cache.page_size + keys - 1) / keys + kPagedSegTiles;
-  const int64_t rows = (int64_t)a.n_req * a.cache.n_kv_heads;
+  const int G = a.n_heads / a.cache.n_kv_heads, run = paged_attention_group(G, hd, a.cache.dtype == SX_DTYPE_F32);
+  const int64_t rows = (int64_t)a.n_req * a.cache.n_kv_heads * ((G + run - 1) / run);
   return rows > INT64_MAX / tiles ? INT64_MAX : rows * tiles;
 }
 
@@ -237,7 +237,7 @@ int sx_paged_attention_workspace(int32_t n_heads, int32_t n_kv_heads, int32_t he
                                  size_t* bytes_out) {
   return guarded([&]() -> int {
     if (!bytes_out) return refuse(SX_E_INVALID, "sx_paged_attention_workspace: null argument");
-    if (n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads || n_heads / n_kv_heads > 16 ||
+    if (n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads || n_heads > (1 << 16) ||
         (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256))
       return refuse(SX_E_UNSUPPORTED, "sx_paged_attention_workspace: heads or head_dim not supported");
     const int sms = paged_sms(device);

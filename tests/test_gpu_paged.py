@@ -148,6 +148,16 @@ def test_attend_short_and_odd_lengths(paged, qt, ct, H, hkv, hd):
 
 
 @pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("H,hkv,hd", [(17, 1, 64), (71, 1, 64), (66, 2, 128), (9, 1, 256), (40, 2, 256), (24, 1, 32), (128, 1, 128)])
+def test_attend_wide_groups_are_run_in_parts(paged, qt, ct, H, hkv, hd):
+    lens = [0, 1, 40, 333, 2500]
+    k, v, table = filled(lens, hkv, 16, hd, DT[ct], "nhd", 3)
+    q = torch.randn((len(lens), H, hd), generator=gen(3), device="cuda").to(DT[qt])
+    assert_attends(paged, q, k, v, table, lens, 16, "nhd")
+    assert_attends(paged, q[:3], k, v, table, lens[:3], 16, "nhd", max_len=40)
+
+
+@pytest.mark.parametrize("qt,ct", TYPES)
 @pytest.mark.parametrize("n,H,hkv,hd,ps", [(1, 32, 8, 128, 64), (1, 8, 1, 64, 8), (3, 14, 2, 64, 16), (2, 4, 4, 256, 128),
                                             (5, 16, 1, 128, 32), (1, 2, 1, 32, 1024)])
 def test_attend_long_lengths_are_split_and_joined(paged, qt, ct, n, H, hkv, hd, ps):
@@ -403,8 +413,7 @@ def test_attend_refusals(paged):
         with pytest.raises(ValueError):
             bad()
     for bad in (lambda: paged.attend(q[:, :3], k, v, table, d), lambda: paged.attend(q.half(), k, v, table, d),
-                lambda: paged.attend(q, k, v, table, d, workspace=torch.empty(8, device="cuda")),
-                lambda: paged.attend(torch.randn(1, 34, 64, device="cuda"), k, v, table, d)):
+                lambda: paged.attend(q, k, v, table, d, workspace=torch.empty(8, device="cuda"))):
         with pytest.raises(sx.SyrinxError):
             bad()
     assert paged.attend(q[:0], k, v, table, d).shape == (0, 4, 64)

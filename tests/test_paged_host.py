@@ -89,7 +89,7 @@ ATTENTION = [
     (dict(q=None), INVALID), (dict(out=None), INVALID), (dict(table=None), INVALID), (dict(lens=None), INVALID),
     (dict(workspace_bytes=0), RANGE), (dict(workspace=P + 4), INVALID),
     (dict(n_req=-1), INVALID), (dict(q_dtype=1), UNSUPPORTED), (dict(n_heads=0), UNSUPPORTED),
-    (dict(n_heads=33), UNSUPPORTED), (dict(n_heads=136), UNSUPPORTED), (dict(table_width=0), INVALID),
+    (dict(n_heads=33), UNSUPPORTED), (dict(n_heads=1 << 17), RANGE), (dict(table_width=0), INVALID),
     (dict(table_stride=15), INVALID), (dict(max_len=-1), INVALID), (dict(q_stride=31 * 128), INVALID),
     (dict(out_stride=32 * 128 + 4), INVALID), (dict(q=P + 8), INVALID), (dict(table_width=1 << 26, table_stride=1 << 26), RANGE),
     (dict(n_req=1 << 29), RANGE),
@@ -119,12 +119,6 @@ def test_append_refuses(kw, code):
 def test_attention_refuses(kw, code):
     rc, msg = call("sx_paged_attention", attention_args(**kw))
     assert rc == code and "sx_paged_attention" in msg
-
-
-def test_wide_groups_refused_where_they_do_not_fit():
-    rc, _ = call("sx_paged_attention", attention_args(c=dict(head_dim=256, token_stride=256), n_heads=128, q_stride=1 << 16,
-                                                      out_stride=1 << 16))
-    assert rc == UNSUPPORTED
 
 
 def test_null_arguments_and_devices():
