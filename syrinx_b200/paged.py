@@ -66,11 +66,6 @@ def _ints(dev: int, t: torch.Tensor, name: str, least: int) -> int:
     raise ValueError(f"{name}: a contiguous int32 tensor of at least {least} entries on the same CUDA device")
 
 
-def _row(t: torch.Tensor) -> int:
-    """Elements from one row to the next (of a single row: its own)."""
-    return t.stride(0) if t.shape[0] > 1 else t.numel()
-
-
 def _table(dev: int, t: torch.Tensor, n: int) -> tuple:
     """Address, elements from row to row and pages a row of a block table."""
     s = t.shape
@@ -129,32 +124,36 @@ def append(x, k, v, slots, *, n_heads: int, positions=None, cos=None, sin=None, 
     Keys and values go to `k` / `v` at `slots`; the query heads are returned, in `out` [rows, n_heads *
     head_dim] where it is given. Rows with slot -1 are left out of both."""
     cache = _cache(k, v, layout)
-    rows, width = x.shape
+    (rows, width), (x_row, x_step) = x.shape, x.stride()
     hkv, hd, dtype = cache[8], cache[9], x.dtype
-    _need(dtype in _DTYPES and x.stride(1) == 1, "x: floating [rows, heads * head_dim]")
-    _need(width == (n_heads + 2 * hkv) * hd, "x: a row is n_heads + 2 kv heads of head_dim")
+    q_width = n_heads * hd
+    if dtype not in _DTYPES or x_step != 1 or width != q_width + 2 * hkv * hd:
+        raise ValueError("x: floating [rows, (n_heads + 2 kv heads) * head_dim], rows contiguous")
     if out is None:
-        out = torch.empty((rows, n_heads * hd), dtype=dtype, device=x.device)
-    elif out.dim() != 2 or out.shape[0] < rows or out.shape[1] != n_heads * hd or out.dtype is not dtype or (
-            out.stride(1) != 1 and out.shape[1] > 1):
-        raise ValueError("out: [rows, n_heads * head_dim] of x's type")
+        out = torch.empty((rows, q_width), dtype=dtype, device=x.device)
+    q_rows, q_row, q_step = *out.shape[:1], *out.stride()
+    if out.shape[1] != q_width or q_rows < rows or out.dtype is not dtype or (q_step != 1 and q_width > 1):
+        raise ValueError("out: [rows, n_heads * head_dim] of x's type, rows contiguous")
+    if rows < 2:  # the one row's stride says nothing
+        x_row, q_row = width, q_width
     dev = x.get_device()
     _on(dev, k, v, cos, sin, q_norm, k_norm, out)
     n_pos = 0
     if cos is not None or sin is not None:
-        _need(cos is not None and sin is not None and cos.dtype is _F32 and sin.dtype is _F32
-              and cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == hd // 2 and cos.is_contiguous()
-              and sin.is_contiguous(), "cos and sin: float32 [positions, head_dim / 2]")
-        n_pos = cos.shape[0]
+        if (cos is None or sin is None or cos.dtype is not _F32 or sin.dtype is not _F32 or not cos.is_contiguous()
+                or not sin.is_contiguous() or sin.shape != (table := cos.shape) or len(table) != 2
+                or table[1] != hd // 2):
+            raise ValueError("cos and sin: float32 [positions, head_dim / 2]")
+        n_pos = table[0]
     for t in (q_norm, k_norm):
-        _need(t is None or (t.dtype is _F32 and t.numel() == hd and t.is_contiguous()),
-              "q_norm and k_norm: float32 [head_dim]")
+        if t is not None and (t.dtype is not _F32 or t.numel() != hd or not t.is_contiguous()):
+            raise ValueError("q_norm and k_norm: float32 [head_dim]")
     args = _APPEND_ARGS.pack(
         *cache, x.data_ptr(), out.data_ptr() if n_heads else 0, _ints(dev, slots, "slots", rows),
         0 if positions is None else _ints(dev, positions, "positions", rows), cos.data_ptr() if n_pos else 0,
         sin.data_ptr() if n_pos else 0, 0 if q_norm is None else q_norm.data_ptr(),
         0 if k_norm is None else k_norm.data_ptr(), 0 if status is None else _ints(dev, status, "status", 1),
-        _row(x), _row(out), eps, _DTYPES[dtype], rows, n_heads, n_pos, int(interleaved))
+        x_row, q_row, eps, _DTYPES[dtype], rows, n_heads, n_pos, int(interleaved))
     _lib.check(_lib.lib().sx_paged_append(args, dev, _stream(dev)))
     return out
 
@@ -179,13 +178,21 @@ def attend(q, k, v, table, lens, *, scale: float | None = None, layout: str = "h
     hkv, hd, dtype, shape = cache[8], cache[9], q.dtype, q.shape
     if len(shape) != 3 or shape[2] != hd or dtype not in _DTYPES:
         raise ValueError("q: floating [requests, heads, head_dim]")
-    n, heads = shape[0], shape[1]
-    if q.stride(2) != 1 or (heads > 1 and q.stride(1) != hd):
+    n, heads, _ = shape
+    q_row, q_head, q_step = q.stride()
+    if q_step != 1 or (q_head != hd and heads > 1):
         raise ValueError("q: a request's heads must be contiguous")
     if out is None:
         out = torch.empty((n, heads, hd), dtype=dtype, device=q.device)
-    elif out.shape != shape or out.dtype is not dtype or out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd):
-        raise ValueError("out: q's shape and type, a request's heads contiguous")
+        out_row = heads * hd
+    else:
+        if out.shape != shape or out.dtype is not dtype:
+            raise ValueError("out: q's shape and type")
+        out_row, out_head, out_step = out.stride()
+        if out_step != 1 or (out_head != hd and heads > 1):
+            raise ValueError("out: a request's heads must be contiguous")
+    if n == 1:  # the one row's stride says nothing
+        q_row = out_row = heads * hd
     dev = q.get_device()
     _on(dev, k, v, out, lse, workspace)
     if n == 0:
@@ -204,7 +211,7 @@ def attend(q, k, v, table, lens, *, scale: float | None = None, layout: str = "h
     args = _ATTEND_ARGS.pack(
         *cache, q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), address,
         _ints(dev, lens, "lens", n), 0 if status is None else _ints(dev, status, "status", 1), pointer, size,
-        _row(q), _row(out), stride, width, n, heads, _DTYPES[dtype], max_len, hd ** -0.5 if scale is None else scale)
+        q_row, out_row, stride, width, n, heads, _DTYPES[dtype], max_len, hd ** -0.5 if scale is None else scale)
     _lib.check(_lib.lib().sx_paged_attention(args, dev, _stream(dev)))
     return out
 
