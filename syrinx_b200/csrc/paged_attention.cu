@@ -719,7 +719,8 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
   Place<M> pc, last = {};  // this warp's run: [pc, last)
   uint32_t share = 1;  // cost per CTA
   bool some_empty = false;
-  if (tid < 2 * NW) sm.piece[tid].z = 0;
+  if (lane < 2) sm.piece[2 * warp + lane].z = 0;  // each warp its own: nothing orders the warps yet
+  __syncwarp();
 
   // requests without keys get their result at once
   auto nothing = [&](long long i) {

@@ -60,6 +60,7 @@ int paged_check(const sx_paged_plan_args& a) {
     return refuse(SX_E_UNSUPPORTED, "sx_paged_plan: page_size must be a power of two, 8 .. 1024");
   if (a.n_pages < 1 || a.table_width < 1 || a.max_tokens < 0 || a.reserved != 0)
     return refuse(SX_E_INVALID, "sx_paged_plan: non-positive pages or table width, negative max_tokens, or reserved is not 0");
+  if (a.max_tokens > INT32_MAX - 4) return refuse(SX_E_RANGE, "sx_paged_plan: max_tokens must be below 2^31 - 4");
   if (a.max_tokens > 0 && !a.slots) return refuse(SX_E_INVALID, "sx_paged_plan: null slots");
   if (a.max_tokens == 0 && (a.slots || a.tok_seq || a.tok_pos))
     return refuse(SX_E_INVALID, "sx_paged_plan: token arrays without max_tokens");
@@ -111,7 +112,7 @@ int paged_check(const sx_paged_attention_args& a, int sms) {
     return refuse(SX_E_RANGE, "sx_paged_attention: a row's positions must be below 2^31");
   if ((int64_t)a.n_req * a.n_heads > INT32_MAX)
     return refuse(SX_E_RANGE, "sx_paged_attention: n_req * n_heads must be below 2^31");
-  if (paged_attention_cost(a) > UINT32_MAX)
+  if (paged_attention_cost(a) > UINT32_MAX - (1 << 16))
     return refuse(SX_E_RANGE, "sx_paged_attention: requests x kv heads x a row's positions is too large for one call");
   const int64_t width = (int64_t)a.n_heads * c.head_dim;
   if ((rc = check_row(a.q, a.q_stride, width, a.q_dtype, "sx_paged_attention: q"))) return rc;

@@ -64,7 +64,7 @@ PLAN = [
     (dict(lens_in=None), INVALID), (dict(delta=None), INVALID), (dict(n_free_in=None), INVALID),
     (dict(lens_out=None), INVALID), (dict(n_free_out=None), INVALID), (dict(table=None), INVALID),
     (dict(free_pages=None), INVALID), (dict(status=None), INVALID), (dict(slots=None), INVALID),
-    (dict(max_tokens=0), INVALID), (dict(max_tokens=-1), INVALID), (dict(n_req=0), RANGE), (dict(n_req=8193), RANGE),
+    (dict(max_tokens=0), INVALID), (dict(max_tokens=-1), INVALID), (dict(max_tokens=2 ** 31 - 1), RANGE), (dict(n_req=0), RANGE), (dict(n_req=8193), RANGE),
     (dict(page_size=48), UNSUPPORTED), (dict(page_size=4), UNSUPPORTED), (dict(page_size=2048), UNSUPPORTED),
     (dict(n_pages=0), INVALID), (dict(table_width=0), INVALID), (dict(table_stride=31), INVALID),
     (dict(n_pages=1 << 26), RANGE), (dict(reserved=1), INVALID),
@@ -92,7 +92,7 @@ ATTENTION = [
     (dict(n_heads=33), UNSUPPORTED), (dict(n_heads=1 << 17), RANGE), (dict(table_width=0), INVALID),
     (dict(table_stride=15), INVALID), (dict(max_len=-1), INVALID), (dict(q_stride=31 * 128), INVALID),
     (dict(out_stride=32 * 128 + 4), INVALID), (dict(q=P + 8), INVALID), (dict(table_width=1 << 26, table_stride=1 << 26), RANGE),
-    (dict(n_req=1 << 29), RANGE),
+    (dict(n_req=1 << 29), RANGE), (dict(n_req=1 << 20, table_width=1 << 15, table_stride=1 << 15), RANGE),
 ]
 
 
