@@ -137,8 +137,9 @@ int sx_paged_append(const sx_paged_append_args* args, int32_t device, void* cuda
  * zeros; either sets *status (nullable) to SX_E_RANGE, which is not written otherwise.
  *
  * The key axis of all requests is cut into even shares for the GPU's SMs (so the last bits of
- * a result depend on the lengths of all of them); partial results pass through `workspace`, whose content means nothing before and after the call. Calls that
- * may run at the same time (on two streams, or two captured graphs) need a workspace each.
+ * a result depend on the lengths of all of them); partial results pass through `workspace`,
+ * whose content means nothing before and after the call. Calls that may run at the same time
+ * (on two streams, or two captured graphs) need a workspace each. `out` may be `q` itself.
  */
 typedef struct sx_paged_attention_args {
   sx_paged_cache cache;

@@ -303,6 +303,64 @@ def test_attend_strided_rows_and_neighbours_left_alone(paged):
     assert (wide[:, 0] == 5).all() and (wide[:, 9] == 5).all()
 
 
+@pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("lens,H,hkv", [([1, 0, 60, 130], 8, 2), ([9000], 8, 2), ([700, 0, 1, 3000, 33] * 30, 8, 2),
+                                        ([400] * 9, 40, 1)])
+def test_attend_over_its_own_queries(paged, qt, ct, lens, H, hkv):
+    """out may be q: in one CTA per request, split and joined, and with several groups a kv head."""
+    k, v, table = filled(lens, hkv, 32, 64, DT[ct], "hnd", 41)
+    q = torch.randn((len(lens), H, 64), generator=gen(42), device="cuda").to(DT[qt])
+    d = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = paged.attend(q, k, v, table, d)
+    got = q.clone()
+    assert paged.attend(got, k, v, table, d, out=got) is got
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("requests", [2, 40])
+def test_first_calls_of_a_process_can_be_captured(requests):
+    """Nothing of a call has to have run before it is captured: a new process captures its first plan,
+    append (of few and of many rows) and attention, and the replay equals calls made afterwards."""
+    import os
+    import subprocess
+    import sys
+
+    code = f"""
+import torch
+from syrinx_b200 import paged
+n, H, hkv, hd, ps, width = {requests}, 32, 8, 128, 16, 40
+g0 = torch.Generator(device="cuda"); g0.manual_seed(3)
+k = torch.randn(n * width + 200, hkv, ps, hd, generator=g0, device="cuda").bfloat16()
+v = torch.randn(k.shape, generator=g0, device="cuda").bfloat16()
+lens = torch.arange(1, n + 1, dtype=torch.int32, device="cuda") % 20 * ps  # every request needs a page
+table = torch.arange(n * width, dtype=torch.int32, device="cuda").view(n, width).contiguous()
+free = torch.arange(k.shape[0], dtype=torch.int32, device="cuda").roll(200)  # the spare pages lie lowest
+left = torch.full((1,), n, dtype=torch.int32, device="cuda")
+delta, slots = torch.ones_like(lens), torch.empty_like(lens)
+x = torch.randn((n, (H + 2 * hkv) * hd), generator=g0, device="cuda").bfloat16()
+spare = torch.arange((n * width + 100) * ps, (n * width + 200) * ps, dtype=torch.int32, device="cuda")
+many = torch.randn((spare.numel(), (H + 2 * hkv) * hd), generator=g0, device="cuda").bfloat16()
+work = torch.empty(paged.workspace_bytes(H, hkv, hd), dtype=torch.uint8, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    status = paged.plan(lens, delta, table, free, left, page_size=ps, slots=slots)
+    q = paged.append(x, k, v, slots, n_heads=H)
+    q2 = paged.append(many, k, v, spare, n_heads=H)
+    out = paged.attend(q.view(n, H, hd), k, v, table, lens, workspace=work)
+graph.replay()
+torch.cuda.synchronize()
+assert status.tolist() == [0, n, n, 0], status.tolist()
+assert torch.equal(q, x[:, : H * hd])
+assert torch.equal(q2, many[:, : H * hd])
+assert torch.equal(out, paged.attend(q.view(n, H, hd), k, v, table, lens))
+print("same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("same"), r.stderr[-2000:]
+
+
 @pytest.mark.parametrize("ct", ["bf16", "f32"])
 def test_attend_offsets_past_32_bits(paged, ct):
     """Pages whose elements lie beyond 2^31 (and bytes beyond 2^32) from the base."""
