@@ -182,12 +182,17 @@ __device__ __forceinline__ void split16(float lo, float hi, uint32_t (&w)[NL]) {
 }
 
 // The same for weights, which are not negative: every part but the last is cut off, not rounded,
-// and none that is left over is zero (2^-30 of the weight at least, 2^-22 in f16), so that an
-// infinite value times the parts is infinite and not inf - inf or 0 inf.
+// and no part of a weight above zero is zero, so that an infinite value times the parts is
+// infinite and not inf - inf or 0 inf. A part is the type's least at least: f16's 2^-24 (2^-39 of
+// the largest weight, which is 2^kLift), in bf16, whose range is f32's, 2^-126. (A floor in
+// proportion to the weight, 2^-22 of it in f16, was below 2^-24 for weights under 2^-12.)
 template <typename T, int NP>
 __device__ __forceinline__ void split_weights(float lo, float hi, uint32_t (&w)[NP]) {
   constexpr bool f16 = std::is_same<T, __half>::value;
-  const float least_lo = lo * (f16 ? 0x1p-22f : 0x1p-30f), least_hi = hi * (f16 ? 0x1p-22f : 0x1p-30f);
+  // 0 for 0: pow2 gives nothing else below 2^-126
+  const float least_lo = fminf(f16 ? lo * 0x1p102f : lo, f16 ? 0x1p-24f : 0x1p-126f);
+  const float least_hi = fminf(f16 ? hi * 0x1p102f : hi, f16 ? 0x1p-24f : 0x1p-126f);
+  if constexpr (f16) lo = fmaxf(lo, least_lo), hi = fmaxf(hi, least_hi);
 #pragma unroll
   for (int x = 0; x < NP; x++) {
     if (x + 1 == NP) {
@@ -226,8 +231,9 @@ struct Mma {
   // of the result, where a single value would add a rounding as large as the result's own.
   static constexpr int NL = kQ32 ? (kF16 ? 2 : 3) : 1;
   static constexpr int NP = kQ32 ? (kF16 ? 2 : 3) : 2;
-  // f16 weights are kept as 2^10 p, so that their low parts stay above f16's smallest step
-  static constexpr float kLift = kF16 ? 10.f : 0.f;
+  // f16 weights are kept as 2^15 p, at the top of f16's range, so that as much as can be of their
+  // low parts is above f16's smallest step
+  static constexpr float kLift = kF16 ? 15.f : 0.f;
 
   uint32_t q[NT][NL][KS][2];
   float o[NT][KS][4];
