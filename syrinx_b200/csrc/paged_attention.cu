@@ -149,6 +149,35 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
 }
+// The same with nothing to add to: d = a b. The tensor core cuts off what lies below the last place
+// of the largest term, sums included (measured: towards zero every time, 0.9 steps on average and
+// 2.3 at most where the sum is 100 times the product, 3.5 at 1000 times), so a sum that ran through
+// a thousand products would drift by that much each time: 460 u (u = 2^-24) over a run of 16384 keys,
+// 1600 at head_dim 256. Products start from zero therefore and are added in f32: 3 to 18 u.
+template <typename T>
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+  }
+}
+// x + d, and x f + d with f of elements 0 and 2 in f[0], of 1 and 3 in f[1].
+__device__ __forceinline__ void add4(float (&x)[4], const float (&d)[4]) {
+#pragma unroll
+  for (int c = 0; c < 4; c += 2) unpack2(add2(pack2(x[c], x[c + 1]), pack2(d[c], d[c + 1])), x[c], x[c + 1]);
+}
+__device__ __forceinline__ void fma4(float (&x)[4], const float (&f)[2], const float (&d)[4]) {
+#pragma unroll
+  for (int c = 0; c < 4; c += 2)
+    unpack2(fma2(pack2(x[c], x[c + 1]), pack2(f[0], f[1]), pack2(d[c], d[c + 1])), x[c], x[c + 1]);
+}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -237,7 +266,7 @@ struct Mma {
 
   uint32_t q[NT][NL][KS][2];
   float o[NT][KS][4];
-  float m[NT][2], l[NT][2], sl2[NT][2];
+  float m[NT][2], l[NT][2], lost[NT][2], sl2[NT][2];  // lost: what rounding has added to l
 
   static __device__ __forceinline__ uint32_t at(int row, int chunk) {  // byte of a 16-byte chunk in a tile
     if constexpr (CPR == 4) return row * RB + ((chunk ^ ((row >> 1) & 3)) << 4);
@@ -296,7 +325,7 @@ struct Mma {
       for (int c = 0; c < 2; c++) {
         sl2[nt][c] = __shfl_sync(0xffffffffu, mine, 4 * (2 * t + c));
         m[nt][c] = -INFINITY;
-        l[nt][c] = 0.f;
+        l[nt][c] = lost[nt][c] = 0.f;
       }
 #pragma unroll
       for (int j = 0; j < KS; j++)
@@ -314,17 +343,26 @@ struct Mma {
     for (int mt = 0; mt < MT; mt++) {
       float low[NT][4];  // the products of a split query's lower parts
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) s[mt][nt][c] = low[nt][c] = 0.f;
-#pragma unroll
       for (int ks = 0; ks < KS; ks++) {
         uint32_t a[4];
         ldsm4(a, ks_ + at(mt * 16 + r16, 2 * ks + c1));
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++) {
+          if (ks == 0) {
+            mma16816_first<CT>(s[mt][nt], a, q[nt][0][ks][0], q[nt][0][ks][1]);
+          } else {
+            float d[4];
+            mma16816_first<CT>(d, a, q[nt][0][ks][0], q[nt][0][ks][1]);
+            add4(s[mt][nt], d);
+          }
 #pragma unroll
-          for (int y = 0; y < NL; y++) mma16816<CT>(y ? low[nt] : s[mt][nt], a, q[nt][y][ks][0], q[nt][y][ks][1]);
+          for (int y = 1; y < NL; y++) {  // 2^-8 of the score at most: their sum may lose a few bits
+            if (ks == 0 && y == 1)
+              mma16816_first<CT>(low[nt], a, q[nt][y][ks][0], q[nt][y][ks][1]);
+            else
+              mma16816<CT>(low[nt], a, q[nt][y][ks][0], q[nt][y][ks][1]);
+          }
+        }
       }
       if constexpr (NL > 1) {
         // an infinite key makes the lower parts' products infinite too, of either sign
@@ -335,7 +373,6 @@ struct Mma {
       }
     }
     uint32_t p[MT][NT][NP][2];
-    bool turned = false;
     float alpha[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -354,17 +391,16 @@ struct Mma {
         top[c] = fmaxf(top[c], m[nt][c]);
         const float ref = finite_or_zero(top[c]);
         alpha[nt][c] = pow2(m[nt][c] - ref);
-        turned |= alpha[nt][c] != 1.f;
         m[nt][c] = top[c];
         top[c] = ref - kLift;
-        l[nt][c] *= alpha[nt][c];
       }
+      float sum[2] = {0.f, 0.f};  // of the tile's weights
 #pragma unroll
       for (int mt = 0; mt < MT; mt++) {
 #pragma unroll
         for (int c = 0; c < 4; c++) {
           s[mt][nt][c] = pow2(s[mt][nt][c] - top[c & 1]);
-          l[nt][c & 1] += s[mt][nt][c];
+          sum[c & 1] += s[mt][nt][c];
         }
         uint32_t lo[NP], hi[NP];
         split_weights<CT, NP>(s[mt][nt][0], s[mt][nt][1], lo);
@@ -375,14 +411,13 @@ struct Mma {
           p[mt][nt][y][1] = transpose8x8(hi[y]);
         }
       }
-    }
-    if (__any_sync(0xffffffffu, turned)) {
+      // equal weights are rounded the same way tile after tile: what an addition loses goes to the next
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int j = 0; j < KS; j++)
-#pragma unroll
-          for (int c = 0; c < 4; c++) o[nt][j][c] *= alpha[nt][c & 1];
+      for (int c = 0; c < 2; c++) {
+        const float old = l[nt][c] * alpha[nt][c], x = fmaf(-lost[nt][c], alpha[nt][c], sum[c]);
+        l[nt][c] = old + x;
+        lost[nt][c] = (l[nt][c] - old) - x;
+      }
     }
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
@@ -392,9 +427,16 @@ struct Mma {
         // rows: keys (lane & 7) + 8 (lane / 16); chunks: elements 16 j + 8 ((lane / 8) & 1)
         ldsm4_t(a, vs_ + at(mt * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * j + ((lane >> 3) & 1)));
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++) {
+          float d[4];  // the weights' lower parts first: what a product cuts off is below the whole's last bits
+          mma16816_first<CT>(d, a, p[mt][nt][NP - 1][0], p[mt][nt][NP - 1][1]);
 #pragma unroll
-          for (int y = 0; y < NP; y++) mma16816<CT>(o[nt][j], a, p[mt][nt][y][0], p[mt][nt][y][1]);
+          for (int y = NP - 2; y >= 0; y--) mma16816<CT>(d, a, p[mt][nt][y][0], p[mt][nt][y][1]);
+          if (mt == 0)
+            fma4(o[nt][j], alpha[nt], d);
+          else
+            add4(o[nt][j], d);
+        }
       }
   }
 

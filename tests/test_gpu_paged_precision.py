@@ -1,5 +1,9 @@
 """What sx_paged_attention's arithmetic holds over 16-bit pages on a B200, against float64.
-u = 2^-24 is half a step of f32."""
+u = 2^-24 is half a step of f32.
+
+A tensor-core product of 16 terms cuts the terms off (and what it adds them to) at the last place
+of the largest one, always towards zero, so one result is off by at most 17 quarter steps, 9 u of
+its terms' sizes, where nothing larger is added to."""
 import math
 
 import pytest
@@ -62,3 +66,57 @@ def test_infinite_values_under_small_weights(paged, qt, ct, hd):
         tol = tol[:, rest][:, None]
     err = (out.double() - want[:, None])[:, :, rest].abs()
     assert (err <= tol).all(), float(err.max())
+
+
+@pytest.mark.parametrize("ct", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_sums_over_long_runs_do_not_drift(paged, ct, hd):
+    """A thousand tiles and more in one warp's run, values of one sign: what every tile's addition
+    lost would add up. All keys but the first have one weight p = exp(-0.3), so the result is
+    (v_0 + p sum v) / (1 + p (n - 1)), whose last bits do not depend on p's own rounding.
+
+    Bound. A tile's sum is off by 9 u (above) + 4 u (the weights' split, 2^-22). The T additions
+    of a run are off by at most u of the partial sum each; as independent ones, of variance a third
+    of that squared, they come to u sqrt(T) / 3 of the sum, and six times that are allowed for; the
+    join of the runs, the sum of the weights (the same additions, on one lane) and the quotient are
+    allowed 2 sqrt(T) + 16 once more."""
+    ps, length = 64, 131072
+    g = gen(hd)
+    n = torch.cuda.get_device_properties(0).multi_processor_count  # a CTA's share is one request
+    v = (1 + torch.rand((length // ps, 1, ps, hd), generator=g, device="cuda")).to(DT[ct])
+    k = torch.zeros_like(v)
+    k[:, :, :, 3] = -0.5
+    k[0, 0, 0, 3] = 0.0
+    q = torch.zeros((n, 2, hd), device="cuda")
+    q[:, :, 3] = 0.6
+    table = torch.arange(length // ps, dtype=torch.int32, device="cuda").expand(n, -1).contiguous()
+    lens = torch.full((n,), length, dtype=torch.int32, device="cuda")
+    out = paged.attend(q, k, v, table, lens, scale=1.0)
+    w = torch.full((length, 1), math.exp(0.6 * -0.5), dtype=torch.float64, device="cuda")
+    w[0] = 1.0
+    want = (w * v.view(length, hd).double()).sum(0) / w.sum()
+    keys = (1024 // hd if ct == "f32" else {32: 64, 64: 32}.get(hd, 16))  # of a tile
+    T = length // keys // (4 if hd == 256 and ct != "f32" else 8)
+    err = ((out.double() - want) / want).abs().max()
+    assert err <= (4 * math.sqrt(T) + 13 + 16) * U, f"{float(err / U):.1f} u, {T} tiles"
+
+
+@pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("hd", [32, 64, 128, 256])
+def test_scores_of_one_sign(paged, qt, ct, hd):
+    """A request of one key has lse = scale q.k; all products positive, so that what they lose adds up.
+
+    Bound. The products of 16 elements are cut off by at most 8 u of their sum (above; f32 pages: a
+    product is rounded once), their hd / 16 (f32 pages: hd / 4 and more) additions come to 2 sqrt(hd / 4) u
+    as in the runs above; queries' parts, scale and the two logarithms 8 u."""
+    n, ps = 512, 8
+    g = gen(hd)
+    k = torch.randn((n, 1, ps, hd), generator=g, device="cuda").abs().to(DT[ct])
+    q = torch.randn((n, 4, hd), generator=g, device="cuda").abs().to(DT[qt])
+    table = torch.arange(n, dtype=torch.int32, device="cuda").view(n, 1)
+    lens = torch.ones(n, dtype=torch.int32, device="cuda")
+    lse = torch.empty((n, 4), device="cuda")
+    paged.attend(q, k, torch.zeros_like(k), table, lens, scale=1.0, lse=lse)
+    want = torch.einsum("nhd,nd->nh", q.double(), k[:, 0, 0].double())
+    err = ((lse.double() - want) / want).abs().max()
+    assert err <= (8 + 2 * math.sqrt(hd / 4) + 8) * U, f"{float(err / U):.1f} u"
