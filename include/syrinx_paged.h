@@ -130,7 +130,8 @@ int sx_paged_append(const sx_paged_append_args* args, int32_t device, void* cuda
  * over the lens[i] positions of request i's pages, for kv head h / (n_heads / n_kv_heads).
  * lse[i][h] = log sum_t exp(scale * q.k_t). A request of length 0 gets zeros and -inf, as does
  * a row whose scores are all -inf. Positions behind a request's length are never read. Scores,
- * softmax and sums are f32 whatever the types are. The result does not depend on the other
+ * softmax and sums are f32 whatever the types are; over f16 pages the weights meet the values
+ * with 22 bits, or to 2^-39 of the largest. The result does not depend on the other
  * requests' values; it is the same from call to call.
  *
  * A length beyond table_width pages is cut to it, and a page id outside the cache reads as

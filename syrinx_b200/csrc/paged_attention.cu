@@ -256,10 +256,12 @@ struct Mma {
   static constexpr bool kQ32 = sizeof(QT) == 4;
   // f32 queries and weights pass the tensor cores as sums of 16-bit values: three bf16 hold 24
   // bits; two f16 hold 22, of values that are first scaled to the top of f16's range. 16-bit
-  // queries are exact; their weights keep 16 (bf16) or 22 (f16) bits, far below the rounding
-  // of the result, where a single value would add a rounding as large as the result's own.
+  // queries are exact. Their weights are split the same way, though a 16-bit result would hide two
+  // bf16 values' 16 bits but for its ties: then 32 requests of 8001..32768 keys differ from the
+  // rounded exact result by 1.1e-4 of its size, with three by 2.8e-5 (f32 sums in another order:
+  // 1.05e-4). The third costs nothing up to 8 heads, 10 % at 9 to 16.
   static constexpr int NL = kQ32 ? (kF16 ? 2 : 3) : 1;
-  static constexpr int NP = kQ32 ? (kF16 ? 2 : 3) : 2;
+  static constexpr int NP = kF16 ? 2 : 3;
   // f16 weights are kept as 2^15 p, at the top of f16's range, so that as much as can be of their
   // low parts is above f16's smallest step
   static constexpr float kLift = kF16 ? 15.f : 0.f;

@@ -120,3 +120,34 @@ def test_scores_of_one_sign(paged, qt, ct, hd):
     want = torch.einsum("nhd,nd->nh", q.double(), k[:, 0, 0].double())
     err = ((lse.double() - want) / want).abs().max()
     assert err <= (8 + 2 * math.sqrt(hd / 4) + 8) * U, f"{float(err / U):.1f} u"
+
+
+@pytest.mark.parametrize("qt,ct", [("f32", "bf16"), ("f32", "f16"), ("bf16", "bf16"), ("f16", "f16")])
+def test_weights_keep_their_bits(paged, qt, ct):
+    """Requests of two keys, over many: a 16-bit result is the rounding of one that is f32's but for a few
+    u, so it is off by more than half a step only where the exact result is that near to a tie.
+
+    Bound. The scores are one exact product each, below 4 in size: in units of log 2 they are off by two
+    roundings, so a weight by 4 * 2 u and pow2's own 4 u. Its parts hold 24 bits in bf16 (u), 22 in f16
+    (4 u). Two products (9 u of their sizes), two sums, a quotient: 14 u; and the sum of the weights is
+    off by 12 u. 40 u of sum p|v| / sum p in all, and half a step of the result."""
+    n, H, hd, ps = 4096, 8, 64, 8
+    g = gen(5)
+    k = torch.zeros((n, 1, ps, hd), device="cuda")
+    k[:, 0, 1, 9] = -1.0
+    v = torch.randn((n, 1, ps, hd), generator=g, device="cuda").to(DT[ct])
+    q = torch.zeros((n, H, hd), device="cuda")
+    q[:, :, 9] = 4 * torch.rand((n, H), generator=g, device="cuda")
+    q = q.to(DT[qt])
+    table = torch.arange(n, dtype=torch.int32, device="cuda").view(n, 1)
+    lens = torch.full((n,), 2, dtype=torch.int32, device="cuda")
+    out = paged.attend(q, k.to(DT[ct]), v, table, lens, scale=1.0)
+    p = torch.exp(-q[:, :, 9].double())[:, :, None]
+    a, b = v[:, 0, 0].double()[:, None], v[:, 0, 1].double()[:, None]
+    want = (a + p * b) / (1 + p)
+    tol = 40 * U * (a.abs() + p * b.abs()) / (1 + p)
+    if qt != "f32":
+        step = torch.exp2(torch.floor(torch.log2(out.double().abs()))) * torch.finfo(DT[qt]).eps
+        tol = tol + torch.clamp(step, min=2.0 ** -24 if qt == "f16" else 0.0) / 2
+    over = ((out.double() - want).abs() > tol).sum()
+    assert over == 0, f"{int(over)} of {out.numel()}"
