@@ -296,7 +296,8 @@ int sx_fast_expand_batch_greedy(sx_session* s, const uint32_t* first_codes, cons
                                 int32_t n, uint32_t* codes_out);
 
 /* Device-resident greedy decode of N prefilled sequences for n_frames frames each.
- * frames_out [N x n_frames x (1+C)]; n_frames_out[N] frames produced per sequence. */
+ * frames_out [N x n_frames x (1+C)]; n_frames_out[N] frames produced per sequence: fewer where a
+ * stop id, max_ctx or the page pool ends the loop (sequence i's rows begin at i x n_frames still). */
 int sx_decode_greedy_batch(sx_session* s, int32_t n, int32_t n_frames, int32_t mask_stop,
                            uint32_t* frames_out, int32_t* n_frames_out);
 

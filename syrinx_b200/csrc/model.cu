@@ -1795,6 +1795,7 @@ int run_frames(sx_session* s, int n, int n_frames, int mask_stop, bool sampled, 
     }
     max_len = std::max(max_len, s->len[i]);
   }
+  const int asked = n_frames;  // frames_out holds this many per sequence, however many there is room for
   // each frame's trailing slow step writes position len + f
   n_frames = std::min(n_frames, s->max_ctx - max_len);
   n_frames = std::min(n_frames, s->ring_frames);
@@ -1851,7 +1852,7 @@ int run_frames(sx_session* s, int n, int n_frames, int mask_stop, bool sampled, 
     s->len[i] = lens[i];
     if (frames_out)
       for (int f = 0; f < c; f++)
-        std::memcpy(frames_out + ((size_t)i * n_frames + f) * width, ring.data() + ((size_t)f * s->max_batch + i) * width,
+        std::memcpy(frames_out + ((size_t)i * asked + f) * width, ring.data() + ((size_t)f * s->max_batch + i) * width,
                     width * 4);
   }
   return check_err(s);

@@ -1,0 +1,46 @@
+"""Sessions at the end of their room on a B200: decode loops and calls that meet max_ctx or the
+last page of a pool. Frames and ids are compared for equality with sessions that have room."""
+import numpy as np
+import pytest
+
+import syrinx_b200 as sx
+from syrinx_b200.configs import SX_DTYPE_Q8_0, TINY_S2
+from syrinx_b200.workloads import prompt_for
+
+pytestmark = pytest.mark.gpu
+PAGE = 64
+
+
+@pytest.fixture(scope="module")
+def tiny():
+    m = sx.Model(TINY_S2, sx.synth_blob(TINY_S2, SX_DTYPE_Q8_0, seed=7), device=0)
+    yield m
+    m.close()
+
+
+def prompts(lengths):
+    return [prompt_for(TINY_S2, T, seed=60 + T) for T in lengths]
+
+
+def roomy(m, ps, frames):
+    a = sx.B200DualAr(m, max_ctx=512, max_batch=len(ps))
+    a.prefill_batch(ps)
+    want = a.decode_greedy_batch(len(ps), frames, mask_stop=True)
+    a.close()
+    assert all(len(w) == frames for w in want)
+    return want
+
+
+@pytest.mark.parametrize("how,room", [(dict(max_ctx=512, pool_pages=4), 22), (dict(max_ctx=110), 10),
+                                      (dict(max_ctx=110, pool_pages=8), 10)])
+def test_batched_loop_that_ends_early_keeps_sequences_apart(tiny, how, room):
+    """Three sequences ask for 30 frames where there is room for fewer: each one's frames stand in its
+    own rows. Four pages hold 100 + f, 5 + f and 42 + f positions up to f = 22."""
+    ps = prompts([100, 5, 42])
+    want = roomy(tiny, ps, 30)
+    b = sx.B200DualAr(tiny, max_batch=3, **how)
+    b.prefill_batch(ps)
+    got = b.decode_greedy_batch(3, 30, mask_stop=True)
+    b.close()
+    for g, w in zip(got, want):
+        assert len(g) == room and np.array_equal(g, w[:room])
