@@ -150,8 +150,14 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const sx_paged_plan
   long long v[3] = {0, 0, 0}, sum[3];  // new tokens, pages given back, pages taken
   int err = 0;                         // bit 0: SX_E_INVALID, bit 1: SX_E_RANGE
   int L0 = 0, d0 = 0;                  // one request per thread: kept
+  // Pages that are neither given nor taken but get the first new tokens, the CTAs in turn; the last
+  // one requested is looked at after the sums.
+  unsigned open = 0, highest = 0;
   for (int i = i0; i < i1; i++) {
     const int L = L0 = ld_cg(a.lens_in + i), d = d0 = ld_cg(a.delta + i);
+    highest = max(highest, open);
+    if (d > 0 && L > 0 && (L & (a.page_size - 1)) && (L >> shift) < a.table_width && i % ctas == rank)
+      open = (unsigned)ld_cg(a.table + (size_t)i * a.table_stride + (L >> shift));
     const long long N = max(0ll, (long long)L + d);
     const int h = pages_of(L, shift), m = pages_of(N, shift);
     len[i] = L;
@@ -195,7 +201,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const sx_paged_plan
     const int idx = F + G - 1 - k;
     return idx < F ? ld_cg(a.free_pages + idx) : pushed(idx - F);
   };
-  int page[kKept], wrong = 0;
+  int page[kKept], wrong = max(highest, open) >= (unsigned)a.n_pages;
   if (!err) {
 #pragma unroll
     for (int x = 0; x < kKept; x++) {
