@@ -136,15 +136,15 @@ def append(x, k, v, slots, *, n_heads: int, positions=None, cos=None, sin=None, 
         raise ValueError("out: [rows, n_heads * head_dim] of x's type, rows contiguous")
     if rows < 2:  # the one row's stride says nothing
         x_row, q_row = width, q_width
-    dev = x.get_device()
-    _on(dev, k, v, cos, sin, q_norm, k_norm, out)
     n_pos = 0
     if cos is not None or sin is not None:
         if (cos is None or sin is None or cos.dtype is not _F32 or sin.dtype is not _F32 or not cos.is_contiguous()
                 or not sin.is_contiguous() or sin.shape != (table := cos.shape) or len(table) != 2
-                or table[1] != hd // 2):
-            raise ValueError("cos and sin: float32 [positions, head_dim / 2]")
+                or table[1] != hd // 2 or not table[0]):
+            raise ValueError("cos and sin: float32 [positions, head_dim / 2], one position at least")
         n_pos = table[0]
+    dev = x.get_device()
+    _on(dev, k, v, cos, sin, q_norm, k_norm, out)
     for t in (q_norm, k_norm):
         if t is not None and (t.dtype is not _F32 or t.numel() != hd or not t.is_contiguous()):
             raise ValueError("q_norm and k_norm: float32 [head_dim]")

@@ -41,3 +41,11 @@ def test_plan_checks_the_page_that_a_token_falls_into(paged, n, who, bad):
     where = (delta > 0).nonzero()[:, 0]
     want = table[where, 1] * ps + keep[0][where] % ps
     assert torch.equal(slots[:grown], want.to(torch.int32)) and (slots[grown:] == -1).all()
+
+
+def test_append_refuses_rotation_tables_without_rows(paged):
+    x, none = torch.randn((4, 8 * 64), device="cuda"), torch.zeros((0, 32), device="cuda")
+    k, v = (torch.full((5, 2, 16, 64), 7.0, device="cuda") for _ in range(2))
+    with pytest.raises(ValueError):
+        paged.append(x, k, v, on_gpu([0, 1, 2, 3]), n_heads=4, positions=on_gpu([0, 1, 2, 3]), cos=none, sin=none)
+    assert (k == 7).all() and (v == 7).all()
