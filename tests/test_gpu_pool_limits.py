@@ -44,3 +44,44 @@ def test_batched_loop_that_ends_early_keeps_sequences_apart(tiny, how, room):
     b.close()
     for g, w in zip(got, want):
         assert len(g) == room and np.array_equal(g, w[:room])
+
+
+def test_batched_prefill_and_drive_report_a_failed_reset(tiny):
+    """A reset that fails (its copies are refused on a stream that is being captured) ends the call with
+    its own code; before, the call went on with the lengths and pages of the sequences it was to drop."""
+    import ctypes as C
+
+    torch = pytest.importorskip("torch")
+    cu = C.CDLL("libcuda.so.1")
+    be = sx.B200DualAr(tiny, max_ctx=128, max_batch=2, pool_pages=4)
+    stream = torch.cuda.Stream()
+    be.set_stream(stream.cuda_stream)
+    p = prompts([100, 60])
+    first = be.prefill(p[0]).semantic_logits
+    torch.cuda.synchronize()
+    for call in (lambda: be.prefill_batch([p[1]]), lambda: drive_c(be, p[1], 3)):
+        graph = C.c_void_p()
+        assert cu.cuStreamBeginCapture_v2(C.c_void_p(stream.cuda_stream), 2) == 0
+        try:
+            with pytest.raises(sx.SyrinxError) as e:
+                call()
+        finally:
+            cu.cuStreamEndCapture(C.c_void_p(stream.cuda_stream), C.byref(graph))
+        assert e.value.code == -2 and be.seq_len(0) == 100
+    be.reset()
+    assert be.pool_free() == 4 and np.array_equal(be.prefill(p[0]).semantic_logits, first)
+    be.set_stream(None)
+    be.close()
+
+
+def drive_c(be, prompt, n):
+    """sx_drive with the greedy sampler: [codebooks, frames]."""
+    import ctypes as C
+
+    from syrinx_b200 import _lib
+
+    p = np.ascontiguousarray(prompt, dtype=np.uint32)
+    out, got, params = np.zeros((be.cfg.num_codebooks, max(1, n)), np.uint32), C.c_int32(-1), sx.GREEDY.to_c()
+    _lib.check(_lib.lib().sx_drive(be.handle, p.ctypes.data_as(C.POINTER(C.c_uint32)), p.shape[-1], n, 0, C.byref(params),
+                                   out.ctypes.data_as(C.POINTER(C.c_uint32)), C.byref(got)))
+    return out[:, : got.value]
