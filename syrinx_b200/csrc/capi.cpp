@@ -463,8 +463,7 @@ int sx_drive(sx_session* s, const uint32_t* prompt, int32_t T, int32_t max_frame
       set_error("null codes_out");
       return SX_E_INVALID;
     }
-    rc = session_reset(s);
-    if (rc) return rc;
+    if ((rc = pool_check_prompts(s, &T, 1)) || (rc = session_reset(s))) return rc;
     SemanticConstraint con{d.semantic_begin_id, d.semantic_end_id, d.stop_token_id,
                            d.stop_token_id + (uint32_t)d.num_stop_tokens};
     Sampler smp{SplitMix64{seed}, *params};
@@ -516,8 +515,7 @@ int sx_prefill_batch(sx_session* s, const uint32_t* prompts, const int32_t* lens
       set_error("bad batch");
       return SX_E_INVALID;
     }
-    rc = session_reset(s);
-    if (rc) return rc;
+    if ((rc = pool_check_prompts(s, lens, n)) || (rc = session_reset(s))) return rc;
     size_t off = 0;
     for (int i = 0; i < n; i++) {
       rc = prefill_seq(s, i, prompts + off, lens[i]);

@@ -483,6 +483,14 @@ int pool_reserve(sx_session* s, F&& targets) {
 
 }  // namespace
 
+int pool_check_prompts(const sx_session* s, const int* lens, int n) {
+  int64_t pages = 0;
+  for (int i = 0; s->pool && i < n; i++) pages += (std::max(0, lens[i]) + (int64_t)kPage - 1) / kPage;
+  if (!s->pool || pages <= s->n_pages) return SX_OK;
+  set_error("page pool exhausted: the prompts need " + std::to_string(pages) + " pages of " + std::to_string(s->n_pages));
+  return SX_E_RANGE;
+}
+
 int session_create(sx_model* m, int max_batch, int max_ctx, int kv_dtype, sx_session** out, int pool_pages) {
   if (!m || !out || max_batch < 1 || max_batch > kMaxTok || max_ctx < 1) {
     set_error("sx_session_create: max_batch must be 1..8 and max_ctx >= 1");

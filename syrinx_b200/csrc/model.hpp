@@ -137,6 +137,8 @@ void model_destroy(sx_model* m);
 int session_create(sx_model* m, int max_batch, int max_ctx, int kv_dtype, sx_session** out, int pool_pages = 0);
 void session_destroy(sx_session* s);
 int session_reset(sx_session* s);
+// SX_E_RANGE where the prompts of n sequences do not fit a pooled session that holds nothing else
+int pool_check_prompts(const sx_session* s, const int* lens, int n);
 int sync_lengths(sx_session* s);
 
 // prefill one sequence; leaves its last residual in s->h[seq]

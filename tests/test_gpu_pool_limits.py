@@ -85,3 +85,26 @@ def drive_c(be, prompt, n):
     _lib.check(_lib.lib().sx_drive(be.handle, p.ctypes.data_as(C.POINTER(C.c_uint32)), p.shape[-1], n, 0, C.byref(params),
                                    out.ctypes.data_as(C.POINTER(C.c_uint32)), C.byref(got)))
     return out[:, : got.value]
+
+
+def test_prompts_that_do_not_fit_change_nothing(tiny):
+    """A batched prefill or a drive whose prompts need more pages than the pool has is refused before the
+    sequences that are there are dropped: lengths and free pages stay, and decoding goes on as if it had
+    not been called."""
+    a = sx.B200DualAr(tiny, max_ctx=512, max_batch=2)
+    b = sx.B200DualAr(tiny, max_ctx=512, max_batch=2, pool_pages=4)
+    ps = prompts([100, 20])
+    a.prefill_batch(ps), b.prefill_batch(ps)
+    fa, fb = a.decode_greedy_batch(2, 5, mask_stop=True), b.decode_greedy_batch(2, 5, mask_stop=True)
+    for call in (lambda: b.prefill_batch(prompts([100, 130])), lambda: b.prefill_batch(prompts([257])),
+                 lambda: drive_c(b, prompts([257])[0], 3)):
+        with pytest.raises(sx.SyrinxError) as e:
+            call()
+        assert e.value.code == -7 and [b.seq_len(i) for i in range(2)] == [105, 25] and b.pool_free() == 1
+    fa, fb = a.decode_greedy_batch(2, 7, mask_stop=True), b.decode_greedy_batch(2, 7, mask_stop=True)
+    assert all(np.array_equal(x, y) and len(y) == 7 for x, y in zip(fa, fb))
+    # what fits exactly is taken
+    b.prefill_batch(prompts([128, 127]))
+    assert b.pool_free() == 0
+    a.close()
+    b.close()
