@@ -490,7 +490,7 @@ int sx_drive(sx_session* s, const uint32_t* prompt, int32_t T, int32_t max_frame
       window.push_back(sem);
       if ((int)window.size() > ras_win) window.erase(window.begin());
       if (nf >= max_frames) break;
-      if (pos + 1 >= s->max_ctx) break;
+      if (pos + 1 >= s->max_ctx || !pool_holds(s, 0, pos + 1)) break;
       full[0] = sem;
       for (int c = 0; c < C; c++) full[1 + c] = frame[c];
       const int seq0 = 0;

@@ -491,6 +491,10 @@ int pool_check_prompts(const sx_session* s, const int* lens, int n) {
   return SX_E_RANGE;
 }
 
+bool pool_holds(const sx_session* s, int seq, int positions) {
+  return !s->pool || pool_pages_at(s, [&](int i) { return i == seq ? positions : 0; }) <= s->n_pages;
+}
+
 int session_create(sx_model* m, int max_batch, int max_ctx, int kv_dtype, sx_session** out, int pool_pages) {
   if (!m || !out || max_batch < 1 || max_batch > kMaxTok || max_ctx < 1) {
     set_error("sx_session_create: max_batch must be 1..8 and max_ctx >= 1");

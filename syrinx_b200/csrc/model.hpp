@@ -139,6 +139,8 @@ void session_destroy(sx_session* s);
 int session_reset(sx_session* s);
 // SX_E_RANGE where the prompts of n sequences do not fit a pooled session that holds nothing else
 int pool_check_prompts(const sx_session* s, const int* lens, int n);
+// whether a sequence can grow to that many positions (true in a session without a pool)
+bool pool_holds(const sx_session* s, int seq, int positions);
 int sync_lengths(sx_session* s);
 
 // prefill one sequence; leaves its last residual in s->h[seq]

@@ -36,6 +36,7 @@ def synth_blob(cfg: ModelConfig, wtype: int = SX_DTYPE_Q8_0, seed: int = 0) -> n
 
 
 TP_HANDLE_BYTES = 128  # SX_TP_HANDLE_BYTES
+POOL_PAGE = 64  # positions of a page of a pooled session
 
 
 class Model:
@@ -93,6 +94,7 @@ class B200DualAr:
         self.max_ctx = max_ctx
         self.max_batch = max_batch
         self.kv_dtype = kv_dtype
+        self.pool_pages = pool_pages
         self.handle = C.c_void_p()
         if pool_pages:
             _lib.check(_lib.lib().sx_session_create_pool(model.handle, max_batch, max_ctx, kv_dtype, pool_pages,
@@ -106,6 +108,10 @@ class B200DualAr:
         n = C.c_int32()
         _lib.check(_lib.lib().sx_session_pool_free(self.handle, C.byref(n)))
         return n.value
+
+    def has_page(self, pos: int) -> bool:
+        """Whether sequence 0, `pos` positions long, has a page for its next one, or can take one."""
+        return not self.pool_pages or pos % POOL_PAGE != 0 or self.pool_free() > 0
 
     # -- tensor parallelism ----------------------------------------------------------------
     def tp_handle(self) -> bytes:
@@ -437,7 +443,7 @@ def drive(backend: B200DualAr, prompt: np.ndarray, max_new_frames: int, seed: in
             window.pop(0)
         if len(frames) >= max_new_frames:
             break
-        if pos + 1 >= backend.max_ctx:
+        if pos + 1 >= backend.max_ctx or not backend.has_page(pos):
             break
         step = backend.slow_step([semantic] + frame, pos)
         pos += 1

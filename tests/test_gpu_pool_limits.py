@@ -108,3 +108,19 @@ def test_prompts_that_do_not_fit_change_nothing(tiny):
     assert b.pool_free() == 0
     a.close()
     b.close()
+
+
+@pytest.mark.parametrize("T,n_pages,room", [(100, 2, 29), (64, 1, 1), (120, 3, 40), (1, 1, 40)])
+def test_drive_ends_with_the_pool(tiny, T, n_pages, room):
+    """A drive that meets the last page returns the frames up to there, as at max_ctx: T + f positions
+    after f steps, and a frame more, whose step is not taken."""
+    p = prompts([T])[0]
+    a = sx.B200DualAr(tiny, max_ctx=512)
+    b = sx.B200DualAr(tiny, max_ctx=512, pool_pages=n_pages)
+    want = drive_c(a, p, 40)
+    ended = min(room, want.shape[1])  # a stop id may end both earlier
+    assert ended >= 1
+    for got in (drive_c(b, p, 40), sx.drive(b, p, 40, seed=0, sampling=sx.GREEDY)):
+        assert got.shape[1] == ended and np.array_equal(got, want[:, :ended])
+    a.close()
+    b.close()
