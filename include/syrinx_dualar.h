@@ -150,12 +150,12 @@ int sx_session_create_ex(sx_model* model, int32_t max_batch, int32_t max_ctx, in
  * the memory of what is cached. Block tables, K/V appends and decode attention are the operators
  * of include/syrinx_paged.h, whose attention spreads a sequence over all SMs (one sequence of
  * the 4B shape, f32 cache: 298 frames/s at a context of 512 against 288 in another session,
- * 267 against 194 at 8128). All calls work as on other sessions (greedy output is the same;
- * logits differ in the last bits, since sums are split elsewhere). A call that needs more pages
- * than are free returns SX_E_RANGE and changes nothing (sx_prefill_batch and sx_drive, which begin
- * with a reset, where their prompts need more than the pool has; a sample that
- * sx_slow_step_batch skips counts with its next position too). A decode loop, sx_drive among
- * them, ends early, as at max_ctx, where the pool could run out.
+ * 267 against 194 at 8128). All calls work as on other sessions; logits differ in the last bits,
+ * since sums are split elsewhere, so greedy frames are the same but for codes that nearly tie.
+ * A call that needs more pages than are free returns SX_E_RANGE and changes nothing
+ * (sx_prefill_batch and sx_drive, which begin with a reset, where their prompts need more than
+ * the pool has; a sample that sx_slow_step_batch skips counts with its next position too). A
+ * decode loop, sx_drive among them, ends early, as at max_ctx, where the pool could run out.
  * sx_session_reset returns all pages. Tensor-parallel models: SX_E_UNSUPPORTED. */
 int sx_session_create_pool(sx_model* model, int32_t max_batch, int32_t max_ctx, int32_t kv_dtype,
                            int32_t n_pages, sx_session** out);

@@ -517,7 +517,7 @@ struct Fma {
   static constexpr int LPK = LPK0 < HD / 16 ? HD / 16 : LPK0;
   static constexpr int E = HD / LPK, KG = 32 / LPK;
   static constexpr int NK = TK / KG;           // keys of a tile per lane group
-  static constexpr int KB = GM == 16 || NK < 4 ? 2 : 4;  // keys folded at a time
+  static constexpr int KB = NK < 4 ? 2 : 4;  // keys folded at a time
   static constexpr float kLift = 0.f;
   static_assert(LPK <= 32 && E >= 4 && TK % KG == 0 && NK % KB == 0, "lane split");
 

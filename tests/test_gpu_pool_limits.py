@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import syrinx_b200 as sx
-from syrinx_b200.configs import SX_DTYPE_Q8_0, TINY_S2
+from syrinx_b200.configs import QWEN3_4B, SX_DTYPE_BF16, SX_DTYPE_F32, SX_DTYPE_Q8_0, TINY_S2, shrink
 from syrinx_b200.workloads import prompt_for
 
 pytestmark = pytest.mark.gpu
@@ -124,3 +124,32 @@ def test_drive_ends_with_the_pool(tiny, T, n_pages, room):
         assert got.shape[1] == ended and np.array_equal(got, want[:, :ended])
     a.close()
     b.close()
+
+
+@pytest.mark.parametrize("kv", [SX_DTYPE_F32, SX_DTYPE_BF16])
+def test_hidden_states_at_the_4b_shape(kv):
+    """Four layers of the 4B shape (32 / 8 heads of 128) behind a context of 3000: a pooled session against
+    a static one that is fed the same frames (codes whose logits nearly tie may fall either way).
+
+    Bound. An attention over n positions in another order is off by at most 8 sqrt(n) u = 2.6e-5 of its
+    size, and four layers that pass it on at twice its relative size come to 4e-4 of the hidden state's.
+    A bf16 cache may round a new key the other way, 2^-8 of an element: with |q k| up to 10 and a scale of
+    1 / sqrt(128), a score by 3.5e-3 and, were all the weight on it, the result by as much: 4e-3."""
+    cfg = shrink(QWEN3_4B, 4, 2)
+    m = sx.Model(cfg, sx.synth_blob(cfg, SX_DTYPE_Q8_0, seed=3), device=0)
+    a = sx.B200DualAr(m, max_ctx=4096, kv_dtype=kv)
+    b = sx.B200DualAr(m, max_ctx=4096, kv_dtype=kv, pool_pages=50)
+    prompt = prompt_for(cfg, 40, seed=5)
+    tol = 4e-4 if kv == SX_DTYPE_F32 else 4e-3
+    for be in (a, b):
+        be.fill_kv_synthetic(3000, seed=4)
+    x, y = a.prefill(prompt), b.prefill(prompt)
+    for k in range(60):
+        for p, q in ((x.hidden, y.hidden), (x.semantic_logits, y.semantic_logits)):
+            assert np.max(np.abs(p - q)) <= tol * np.max(np.abs(p))
+        frame, _ = a.frame_step_greedy(None, mask_stop=True)
+        x, y = a.slow_step(frame, 3040 + k), b.slow_step(frame, 3040 + k)
+    assert b.pool_free() == 50 - 49
+    a.close()
+    b.close()
+    m.close()
