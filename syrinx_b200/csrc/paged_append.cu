@@ -530,7 +530,8 @@ cudaError_t launch_t(AppendK a, int sms, cudaStream_t st) {
   cudaLaunchAttribute attr[1];
   // A warp per step up to about three waves of them (48 bf16 heads of 128: 300 rows 4.1 us against
   // 5.6 with the ring, 600 6.2 / 5.9, 1200 10.8 / 8.9, 5000 40 / 25), and for narrow rows, which are
-  // only a few units (14 + 2 x 2 bf16 heads of 64: 5000 rows 8.6 / 11.6, 16384 27.4 / 30.2).
+  // only a few units (14 + 2 x 2 bf16 heads of 64: 5000 rows 8.6 / 11.6, 16384 27.4 / 30.2, where the
+  // bytes alone would take 12.4: a warp has one load in flight and ends).
   if (((long long)a.rows * steps <= 144ll * sms || steps <= 8) && steps <= 65535) {
     constexpr int W = kAppendThreads / 32;
     cudaLaunchConfig_t cfg = launch_cfg(dim3((a.rows + W - 1) / W, steps), dim3(kAppendThreads), 0, st, attr);

@@ -11,23 +11,25 @@
 // enough to read and by latency when there is not.
 //
 // Split. The keys of every (request, kv head) are cut into tiles of 8 KB (16 keys of 128 bf16
-// elements); all tiles of the batch, request by request and head by head, are one line that is
+// elements; 16 KB for 16-bit pages with head_dim 256); all tiles of the batch, request by request and head by head, are one line that is
 // cut into even shares, one per CTA (one CTA per SM), and a CTA's share into even runs, one per
-// warp. However uneven the lengths are, every SM reads the same number of bytes. A warp copies
+// warp. However uneven the lengths are, every SM reads the same number of bytes (requests without
+// keys are not as free: see Place::next). A warp copies
 // its own tiles into a ring of its own (cp.async), so nothing in the main loop waits for
 // another warp, and the ring runs on across the end of one request and the start of the next.
 // A (request, kv head) that lies inside one warp's run is finished by that warp; runs that
 // begin or end inside one leave a partial (m, l, o), joined in shared memory at the end of the
 // CTA, and, where a share begins or ends inside one, through the workspace by a second kernel.
 // Every partial is joined in key order, so results repeat bit for bit. 32 requests of
-// 8001..32768 keys (8 kv heads of 128, bf16, 2.9 GB) take 428 us, 6.76 TB/s; one CTA per (request,
+// 8001..32768 keys (8 kv heads of 128, bf16, 2.9 GB) take 431 us, 6.7 TB/s; one CTA per (request,
 // kv head) took 4630. 64 requests of 1..4099 keys (177 MB) take 37.5 us, of which 10 are what a
 // split call costs before its first tile and after its last one.
 //
 // Products. 16-bit pages: mma.sync.m16n8k16 with the keys as the 16 rows and up to 8 query heads
 // as the 8 columns, S^T = K q^T, then O^T = V^T P^T, so the tiles are A operands as they lie in
 // shared memory (ldmatrix, transposed for V) and an MMA is full for a group of 8; a group of up to
-// 16 takes two. f32 pages would lose precision there; they use packed f32 FMAs, a key's row split
+// 16 takes two. Every product starts from zero and is added in f32 outside the tensor core, which
+// cuts its sums off; values and weights beyond 16 bits go through in parts. f32 pages would lose precision there; they use packed f32 FMAs, a key's row split
 // over a few lanes. A kv head with more query heads than that is run as several groups.
 #include <cuda_runtime.h>
 
@@ -695,6 +697,9 @@ struct Place {
     len = a.n <= kLine && !a.direct ? sm.lens[req] : min(max(ld_cg(a.lens + req), 0), cap);
     tiles = tiles_of<M::TK>(len);
   }
+  // Requests without keys are stepped over one by one: at a read of shared memory each up to kLine
+  // requests, at a load each beyond (5000 requests of which 16 hold 2000 keys: 180 us spread evenly,
+  // 2015 side by side, where the last run walks the rest of the line; 29 without the empty ones).
   __device__ __forceinline__ void next(const AttnK& a, const Smem<M>& sm, int cap) {
     if (++t < tiles) return;
     t = 0;
