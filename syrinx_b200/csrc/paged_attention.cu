@@ -267,6 +267,7 @@ struct Mma {
   // f16 weights are kept as 2^15 p, at the top of f16's range, so that as much as can be of their
   // low parts is above f16's smallest step
   static constexpr float kLift = kF16 ? 15.f : 0.f;
+  static constexpr float kDrop = kF16 ? 0x1p-15f : 1.f;  // 2^-kLift, for the weights' sum
 
   uint32_t q[NT][NL][KS][2];
   float o[NT][KS][4];
@@ -520,7 +521,7 @@ struct Fma {
   static constexpr int E = HD / LPK, KG = 32 / LPK;
   static constexpr int NK = TK / KG;           // keys of a tile per lane group
   static constexpr int KB = NK < 4 ? 2 : 4;  // keys folded at a time
-  static constexpr float kLift = 0.f;
+  static constexpr float kDrop = 1.f;
   static_assert(LPK <= 32 && E >= 4 && TK % KG == 0 && NK % KB == 0, "lane split");
 
   unsigned long long q[GM][E / 2], o[GM][E / 2];
@@ -1006,7 +1007,7 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
             [&](int head, float top, float sum) {
               if (a.lse)
                 a.lse[(size_t)i * a.H + head0 + head] =
-                    sum == 0.f ? -INFINITY : kLn2 * (finite_or_zero(top) + log2f(sum) - M::kLift);
+                    sum == 0.f ? -INFINITY : kLn2 * (finite_or_zero(top) + log2f(sum * M::kDrop));
             });
       } else {
         // a partial: the run's last one may lie in the ring, which is then done with
@@ -1078,7 +1079,7 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
              v.z * inv, v.w * inv);
         if (a.lse && e % (HD / 4) == 0)
           a.lse[(size_t)i * a.H + head0 + head] =
-              sum == 0.f ? -INFINITY : kLn2 * (ref + log2f(sum) - M::kLift);
+              sum == 0.f ? -INFINITY : kLn2 * (ref + log2f(sum * M::kDrop));
       } else {
         reinterpret_cast<float4*>(ws_o)[(size_t)slot * a.G * (HD / 4) + e] = v;
         if (e % (HD / 4) == 0) ws_ml[(size_t)slot * a.G + head] = make_float2(top, sum);
@@ -1093,7 +1094,7 @@ __global__ void __launch_bounds__(M::NW * 32, 1) k_paged_attention(const AttnK a
 // it. Groups of HD / 4 threads take the partials in turn and are added up in order.
 constexpr int kJoinThreads = 128;
 template <int HD, typename QT, bool SHARED>
-__global__ void __launch_bounds__(kJoinThreads) k_paged_join(const AttnK a, int ctas, float lift) {
+__global__ void __launch_bounds__(kJoinThreads) k_paged_join(const AttnK a, int ctas, float drop) {
   constexpr int C = HD / 4, GROUPS = kJoinThreads / C;
   __shared__ float4 acc[kJoinThreads];
   __shared__ float sums[GROUPS], tops[kJoinThreads / 32];
@@ -1153,7 +1154,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_paged_join(const AttnK a, int 
         total == 0.f ? 0.f : __fdiv_rn(x, total));
   }
   if (a.lse && tid == 0)
-    a.lse[(size_t)joint.x * a.H + row] = total == 0.f ? -INFINITY : kLn2 * (ref + log2f(total) - lift);
+    a.lse[(size_t)joint.x * a.H + row] = total == 0.f ? -INFINITY : kLn2 * (ref + log2f(total * drop));
 }
 
 // A CTA per (request, kv head), in one launch, where they are all resident at once and have at
@@ -1188,7 +1189,7 @@ cudaError_t launch_m(AttnK a, long long bound, int sms, cudaStream_t st) {
   e = cudaLaunchKernelEx(&cfg, k_paged_attention<M>, a);
   if (e != cudaSuccess || a.direct) return e;
   cfg = launch_cfg(dim3(sms, a.G), dim3(kJoinThreads), 0, st, attr);
-  return cudaLaunchKernelEx(&cfg, k_paged_join<M::HD, typename M::QT, M::SHARED>, a, sms, M::kLift);
+  return cudaLaunchKernelEx(&cfg, k_paged_join<M::HD, typename M::QT, M::SHARED>, a, sms, M::kDrop);
 }
 
 template <int HD, typename QT, typename CT>

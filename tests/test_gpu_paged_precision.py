@@ -151,3 +151,21 @@ def test_weights_keep_their_bits(paged, qt, ct):
         tol = tol + torch.clamp(step, min=2.0 ** -24 if qt == "f16" else 0.0) / 2
     over = ((out.double() - want).abs() > tol).sum()
     assert over == 0, f"{int(over)} of {out.numel()}"
+
+
+@pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("longest", [40, 6000])
+def test_lse_of_equal_scores(paged, qt, ct, longest):
+    """Scores of zero: lse = log n, whatever power of two the weights are kept at. Their sum is exact, so
+    what is left is log2, half a step and a bit, and a product: 4 u of the result. 6000: joined runs."""
+    hkv, hd, ps = 1, 128, 16
+    lens = list(range(1, 40)) + [longest]
+    pages = -(-longest // ps)
+    k = torch.zeros((pages, hkv, ps, hd), device="cuda").to(DT[ct])
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(len(lens), -1).contiguous()
+    q = torch.randn((len(lens), 4, hd), generator=gen(1), device="cuda").to(DT[qt])
+    lse = torch.empty((len(lens), 4), device="cuda")
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    paged.attend(q, k, k, table, n, lse=lse)
+    want = n.double().log()[:, None]
+    assert ((lse.double() - want).abs() <= 4 * U * want).all(), float(((lse.double() - want).abs() / U).max())
